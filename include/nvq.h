@@ -372,6 +372,46 @@ nvq_status nvq_adamw_step_f32(float* d_param, const float* d_grad, float* d_m, f
                               float bias_corr1, float bias_corr2, float lr, float eps,
                               float lr_times_wd, int apply_decay, int device, void* stream);
 
+/* ---------------------------------------------------------------- embedding
+ * No reference counterpart (NovaNN has no token layers).  Rows are contiguous: table V x D, out and
+ * dout T x D, ids T int32.  Types f32, f16, bf16; any D; buffers aligned to their element (16-byte
+ * alignment and rows of whole 16-byte packets take the fast path).
+ */
+/* out[t] = scale * table[ids[t]], one rounding to the table's type.  An id outside [0, V) gives a row
+ * of zeros and is reported by nvq_device_error_flag (code 71). */
+nvq_status nvq_embedding_fwd(void* d_out, const void* d_table, nvq_dtype dtype, const int32_t* d_ids,
+                             size_t T, size_t V, size_t D, float scale, int device, void* stream);
+/* d_dtable (V x D fp32) = scale * sum of d_dout's rows per id, added in fp32 in the order of t (the same
+ * bits on every call); accumulate != 0 adds to what d_dtable holds (a table that is also the output
+ * projection: its gradient from there first), otherwise rows without a token become 0.  Tokens whose id
+ * is padding_id take no part (a negative padding_id: none is padding); ids outside [0, V) take no part and
+ * are reported (code 71).  D <= 2^22.  Workspace: nvq_embedding_bwd_workspace_bytes, 256-byte aligned,
+ * contents need not be kept or cleared between calls.  More than 131072 tokens run as parts of that
+ * many, one after the other. */
+nvq_status nvq_embedding_bwd_workspace_bytes(size_t T, size_t V, size_t D, size_t* bytes);
+nvq_status nvq_embedding_bwd(float* d_dtable, const void* d_dout, nvq_dtype dout_dtype, const int32_t* d_ids,
+                             size_t T, size_t V, size_t D, float scale, int32_t padding_id, int accumulate,
+                             void* d_workspace, size_t workspace_bytes, int device, void* stream);
+
+/* ---------------------------------------------------------------- gradient norm and clipping
+ * The clipping of SGD (novann/optim/sgd.py:6-87) for any list of tensors.  h_grads, h_counts (elements) and
+ * h_dtypes (nvq_dtype: f32, f16, bf16 or f64, mixed freely) are host arrays of n_tensors entries, read before
+ * the call returns.  Squares are added in fp64, in a fixed order.
+ *   d_norm_coef[0] = norm = sqrt(sum of all squares);  [1] = coef = norm <= max_norm ? 1 : max_norm / norm
+ * nvq_grad_norm writes these two only; nvq_clip_grads also writes out = grad * coef, rounded once to the
+ * tensor's type, to h_out (host array of pointers), or in place where h_out is NULL (then a coefficient of 1
+ * writes nothing).  A NaN norm makes the coefficient NaN, an infinite one 0.  max_norm > 0 (infinity: never
+ * cut).  A tensor may be listed once only, and an output may not overlap another tensor.  Workspace:
+ * nvq_grad_norm_workspace_bytes, 8-byte aligned.
+ */
+nvq_status nvq_grad_norm_workspace_bytes(size_t* bytes);
+nvq_status nvq_grad_norm(float* d_norm_coef, const void* const* h_grads, const size_t* h_counts,
+                         const int32_t* h_dtypes, size_t n_tensors, double max_norm, void* d_workspace,
+                         size_t workspace_bytes, int device, void* stream);
+nvq_status nvq_clip_grads(float* d_norm_coef, void* const* h_out, void* const* h_grads, const size_t* h_counts,
+                          const int32_t* h_dtypes, size_t n_tensors, double max_norm, void* d_workspace,
+                          size_t workspace_bytes, int device, void* stream);
+
 /* ---------------------------------------------------------------- Conv2d forward
  * Replaces F.conv2d, novann/functional.py:275-385: pad (zeros / reflect / replicate /
  * circular = np.pad constant / reflect / edge / wrap) -> im2col with rows ordered (c,kh,kw)

@@ -7,7 +7,7 @@ the library or a GPU is missing.  (``Dropout`` draws its keep mask from NumPy's 
 the host, as the reference does, so that seeded runs drop the same units; ``Flatten`` is a
 reshape.)"""
 from . import functional, quant  # noqa: F401
-from .layers import (BatchNorm1d, BatchNorm2d, Conv2d, Dropout, Flatten, GlobalAvgPool2d,  # noqa: F401
+from .layers import (BatchNorm1d, BatchNorm2d, Conv2d, Dropout, Embedding, Flatten, GlobalAvgPool2d,  # noqa: F401
                      Linear, MaxPool2d, QuantConv2d, QuantLinear, ReLU)
 from .losses import CrossEntropyLoss  # noqa: F401
 from .model import Sequential  # noqa: F401
@@ -19,5 +19,6 @@ register_if_imported()
 
 __all__ = ["functional", "quant", "Linear", "QuantLinear", "ReLU", "Conv2d", "QuantConv2d",
            "BatchNorm1d", "BatchNorm2d", "MaxPool2d", "GlobalAvgPool2d", "Flatten", "Dropout",
+           "Embedding",
            "Sequential", "CrossEntropyLoss", "SGD", "AdamW", "Layer", "Module", "Parameters",
            "register_with_novann"]

@@ -99,6 +99,12 @@ SIGNATURES = {
     "nvq_ce_loss_f32": (i32, [vp, vp, vp, i32, i32, i32, vp]),
     "nvq_sgd_step_f32": (i32, [vp, vp, sz, f32c, f32c, i32, vp]),
     "nvq_adamw_step_f32": (i32, [vp, vp, vp, vp, sz] + [f32c] * 9 + [i32, i32, vp]),
+    "nvq_embedding_fwd": (i32, [vp, vp, i32, vp, sz, sz, sz, f32c, i32, vp]),
+    "nvq_embedding_bwd_workspace_bytes": (i32, [sz, sz, sz, C.POINTER(sz)]),
+    "nvq_embedding_bwd": (i32, [vp, vp, i32, vp, sz, sz, sz, f32c, C.c_int32, i32, vp, sz, i32, vp]),
+    "nvq_grad_norm_workspace_bytes": (i32, [C.POINTER(sz)]),
+    "nvq_grad_norm": (i32, [vp, vp, vp, vp, sz, f64c, vp, sz, i32, vp]),
+    "nvq_clip_grads": (i32, [vp, vp, vp, vp, vp, sz, f64c, vp, sz, i32, vp]),
     "nvq_conv2d_out_size": (i32, [i32] * 8 + [C.POINTER(i32), C.POINTER(i32)]),
     "nvq_im2col_f32": (i32, [vp, vp] + [i32] * 10 + [i32, i32, vp]),
     "nvq_conv2d_fwd_f32": (i32, [vp, vp, vp, vp, vp] + [i32] * 11 + [i32, i32, vp]),

@@ -1,0 +1,567 @@
+// Embedding lookup, out[t] = scale * table[id_t], and the gradient of its table,
+//   dtable[v] = scale * sum over t with id_t == v of dout[t]        (+ dtable[v] when accumulating)
+// added for every v in the order of t, in fp32, without atomics: equal inputs give equal bits.
+#include "packet.cuh"
+
+nvq_status nvq_status_word(int device, int** dev_ptr);
+
+namespace {
+
+enum { ERR_ID_RANGE = 71 };   // an id outside [0, V): recorded for nvq_device_error_flag
+
+// ---------------------------------------------------------------- lookup
+// A group of `lanes` threads (a power of two, at most the block) copies ROWS rows at a time, so that
+// ROWS x (packets per thread) loads are in flight for every id that had to be fetched first.
+constexpr int FWD_THREADS = 256;
+
+template <int DT, int V, int ROWS>
+__global__ void __launch_bounds__(FWD_THREADS)
+embedding_kernel(void* __restrict__ out, const void* __restrict__ table, const int32_t* __restrict__ ids, size_t T,
+                 int vocab, int packets, int lanes_log2, float scale, int* __restrict__ status) {
+    constexpr int BYTES = Packet<DT, V>::BYTES;
+    const int lane = threadIdx.x & ((1 << lanes_log2) - 1);
+    const size_t group = ((size_t)blockIdx.x * FWD_THREADS + threadIdx.x) >> lanes_log2;
+    const size_t t0 = group * ROWS;
+    if (t0 >= T) return;
+    const size_t pitch = (size_t)packets * BYTES;
+    const char* src[ROWS];
+    bool live[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const int id = t0 + r < T ? ids[t0 + r] : 0;
+        live[r] = id >= 0 && id < vocab;
+        if (!live[r] && lane == 0 && status) atomicCAS(status, 0, ERR_ID_RANGE);
+        src[r] = (const char*)table + (live[r] ? (size_t)id : 0) * pitch;
+    }
+    char* dst = (char*)out + t0 * pitch;
+    for (int p = lane; p < packets; p += 1 << lanes_log2) {
+        Packet<DT, V> q[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) q[r].load(src[r] + (size_t)p * BYTES);
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            float f[V];
+            q[r].widen(f);
+#pragma unroll
+            for (int j = 0; j < V; j++) f[j] = live[r] ? f[j] * scale : 0.f;
+            q[r].narrow(f);
+            if (t0 + r < T) q[r].store(dst + r * pitch + (size_t)p * BYTES);
+        }
+    }
+}
+
+template <int DT, int V>
+nvq_status launch_lookup(void* out, const void* table, const int32_t* ids, size_t T, size_t vocab, size_t D,
+                         float scale, int* status, int device, cudaStream_t st) {
+    const int packets = (int)(D / V);
+    int lg = 0;
+    while ((1 << lg) < packets && (1 << lg) < FWD_THREADS) lg++;
+    const size_t groups_per_block = FWD_THREADS >> lg;
+    // four rows per group once that still fills every SM with eight blocks
+    const bool wide = T >= (size_t)4 * 8 * nvq_sm_count(device) * groups_per_block;
+    const size_t per_block = groups_per_block * (wide ? 4 : 1);
+    const size_t grid = (T + per_block - 1) / per_block;
+    if (wide)
+        embedding_kernel<DT, V, 4><<<(unsigned)grid, FWD_THREADS, 0, st>>>(out, table, ids, T, (int)vocab, packets, lg,
+                                                                           scale, status);
+    else
+        embedding_kernel<DT, V, 1><<<(unsigned)grid, FWD_THREADS, 0, st>>>(out, table, ids, T, (int)vocab, packets, lg,
+                                                                           scale, status);
+    NVQ_LAUNCHED();
+    return NVQ_OK;
+}
+
+// the widest packet that divides a row and that both pointers are aligned to
+template <int DT>
+nvq_status lookup(void* out, const void* table, const int32_t* ids, size_t T, size_t vocab, size_t D, float scale,
+                  int* status, int device, cudaStream_t st) {
+    constexpr int V16 = 16 / Elem<DT>::SIZE, V4 = 4 / Elem<DT>::SIZE;
+    if (D % V16 == 0 && nvq_aligned(out, 16) && nvq_aligned(table, 16))
+        return launch_lookup<DT, V16>(out, table, ids, T, vocab, D, scale, status, device, st);
+    if (V4 > 1 && D % V4 == 0 && nvq_aligned(out, 4) && nvq_aligned(table, 4))
+        return launch_lookup<DT, V4>(out, table, ids, T, vocab, D, scale, status, device, st);
+    return launch_lookup<DT, 1>(out, table, ids, T, vocab, D, scale, status, device, st);
+}
+
+// ---------------------------------------------------------------- sorting the tokens
+// The ids of up to SORT_MAX tokens are sorted, stably, with their positions, by one thread-block
+// cluster: each CTA holds a run of at most CTA_ITEMS (id, position) pairs in its shared memory and a
+// pass of least-significant-digit radix sort moves them between the CTAs through distributed shared
+// memory, so that the whole sort is one launch without a global round trip.  The other clusters of the
+// same launch meanwhile clear the gradient table, which takes longer than the sort for any large one.
+constexpr int SORT_THREADS = 1024;
+constexpr int WARPS = SORT_THREADS / 32;
+constexpr int ITEMS = 16;                              // pairs per thread
+constexpr int CTA_ITEMS = SORT_THREADS * ITEMS;
+constexpr int MAX_CLUSTER = 8;
+constexpr int SORT_MAX = CTA_ITEMS * MAX_CLUSTER;      // 131072
+constexpr int MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
+
+struct SortShared {
+    uint2 item[CTA_ITEMS];
+    uint16_t hist[WARPS][MAX_BINS];         // per warp: count, then count of the warps before
+    uint32_t cta_count[MAX_CLUSTER][MAX_BINS];
+    uint32_t base[MAX_BINS];
+    uint32_t scan[WARPS];
+};
+
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+    uint32_t r, a = (uint32_t)__cvta_generic_to_shared(p);
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+struct SortParams {
+    const int32_t* ids;
+    int32_t* sorted_id;      // ids that take no part (padding, out of range) come last, as `vocab`
+    int32_t* sorted_pos;
+    int n, vocab;
+    int padding_id;          // < 0: none
+    int bits, passes;        // digit width and count: passes * bits covers `vocab` itself
+    int chunk_log2;          // pairs per CTA
+    float* clear;            // table to clear, or nullptr
+    size_t clear_floats;
+    int* status;
+};
+
+__global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const SortParams p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    SortShared& sh = *(SortShared*)smem;
+    uint32_t ctas, rank;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (blockIdx.x >= ctas) {               // not the sorting cluster: clear the table
+        const size_t first = (size_t)(blockIdx.x - ctas) * SORT_THREADS + tid;
+        const size_t step = (size_t)(gridDim.x - ctas) * SORT_THREADS;
+        const size_t quads = ((uintptr_t)p.clear & 15) == 0 ? p.clear_floats / 4 : 0;
+        for (size_t i = first; i < quads; i += step) stg_stream_128(p.clear + 4 * i, make_uint4(0, 0, 0, 0));
+        for (size_t i = quads * 4 + first; i < p.clear_floats; i += step) p.clear[i] = 0.f;
+        return;
+    }
+
+    const int chunk = 1 << p.chunk_log2;
+    const int lo = (int)rank << p.chunk_log2;
+    const int count = max(0, min(chunk, p.n - lo));
+    const int bins = 1 << p.bits;
+    // warp w owns items [w * 32 * ITEMS, ...) of the CTA's run, in rounds of 32
+    const int w0 = warp * 32 * ITEMS;
+    uint32_t key[ITEMS], pos[ITEMS];
+    for (int pass = 0; pass < p.passes; pass++) {
+        const int shift = pass * p.bits;
+        for (int i = tid; i < WARPS * MAX_BINS / 2; i += SORT_THREADS) ((uint32_t*)sh.hist)[i] = 0;
+        __syncthreads();
+        uint32_t before[ITEMS / 2];         // 16-bit ranks within the warp's run, packed in pairs
+#pragma unroll
+        for (int r = 0; r < ITEMS; r++) {
+            const int i = w0 + r * 32 + lane;
+            const bool live = i < count;
+            key[r] = 0;
+            pos[r] = 0;
+            if (live) {
+                if (pass == 0) {
+                    const int id = p.ids[lo + i];
+                    const bool inside = id >= 0 && id < p.vocab;
+                    if (!inside && p.status) atomicCAS(p.status, 0, ERR_ID_RANGE);
+                    key[r] = inside && id != p.padding_id ? (uint32_t)id : (uint32_t)p.vocab;
+                    pos[r] = (uint32_t)(lo + i);
+                } else {
+                    const uint2 q = sh.item[i];
+                    key[r] = q.x;
+                    pos[r] = q.y;
+                }
+            }
+            const uint32_t d = live ? (key[r] >> shift) & (bins - 1) : 0xFFFFFFFFu;
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, d);
+            const uint32_t lower = __popc(same & ((1u << lane) - 1u));
+            uint32_t rank_in_warp = 0;
+            if (live) rank_in_warp = sh.hist[warp][d] + lower;
+            __syncwarp();
+            if (live && lower == 0) sh.hist[warp][d] = (uint16_t)(rank_in_warp + __popc(same));
+            __syncwarp();
+            if (r & 1) before[r >> 1] |= rank_in_warp << 16;
+            else before[r >> 1] = rank_in_warp;
+        }
+        __syncthreads();
+        // counts -> counts of the warps before; the CTA's total goes to every CTA of the cluster
+        if (tid < bins) {
+            uint32_t sum = 0;
+            for (int w = 0; w < WARPS; w++) {
+                const uint32_t c = sh.hist[w][tid];
+                sh.hist[w][tid] = (uint16_t)sum;
+                sum += c;
+            }
+            for (uint32_t c = 0; c < ctas; c++)
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.cta_count[rank][tid], c)),
+                             "r"(sum)
+                             : "memory");
+        }
+        cluster_barrier();
+        // first place of each digit among all pairs, plus what the CTAs before this one hold of it
+        uint32_t total = 0, mine = 0;
+        if (tid < bins)
+            for (uint32_t c = 0; c < ctas; c++) {
+                const uint32_t v = sh.cta_count[c][tid];
+                if (c < rank) mine += v;
+                total += v;
+            }
+        uint32_t incl = total;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) sh.scan[warp] = incl;
+        __syncthreads();
+        if (tid < bins) {
+            uint32_t base = incl - total + mine;
+            for (int w = 0; w < warp; w++) base += sh.scan[w];
+            sh.base[tid] = base;
+        }
+        __syncthreads();
+        const bool last = pass == p.passes - 1;
+#pragma unroll
+        for (int r = 0; r < ITEMS; r++) {
+            const int i = w0 + r * 32 + lane;
+            if (i >= count) continue;
+            const uint32_t d = (key[r] >> shift) & (bins - 1);
+            const uint32_t rk = (r & 1) ? before[r >> 1] >> 16 : before[r >> 1] & 0xFFFFu;
+            const uint32_t to = sh.base[d] + sh.hist[warp][d] + rk;
+            if (last) {
+                p.sorted_id[to] = (int32_t)key[r];
+                p.sorted_pos[to] = (int32_t)pos[r];
+            } else {
+                const uint32_t a = cluster_addr(&sh.item[to & (chunk - 1)], to >> p.chunk_log2);
+                asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(key[r]), "r"(pos[r]) : "memory");
+            }
+        }
+        cluster_barrier();       // every pair has landed, and nobody writes here any more at the end
+    }
+}
+
+// ---------------------------------------------------------------- sums over runs of one id
+// A warp adds the rows of PIECE consecutive sorted tokens over a tile of columns.  A run of one id
+// that lies inside the piece goes straight to the table; the two that may cross its ends leave
+// partial sums in `carry` (slot 0: a run that began in an earlier piece, slot 1: one that begins here
+// and goes on), which join_runs_kernel adds up in the order of the pieces.
+constexpr int PIECE = 32;
+constexpr int SUM_WARPS = 4;
+
+template <int DT, int V> struct Tile {
+    static constexpr int NV = (16 / Elem<DT>::SIZE) / V;      // packets per lane: 16 bytes in all
+    static constexpr int E = V * NV;
+    static constexpr int COLS = 32 * E;
+};
+
+// this lane's E sums of columns [c0, c0 + COLS) to (or onto) a row of fp32
+template <int DT, int V>
+__device__ __forceinline__ void put_row(float* row, const float* acc, int c0, int lane, int D, float scale, bool add) {
+    using TL = Tile<DT, V>;
+#pragma unroll
+    for (int k = 0; k < TL::NV; k++) {
+        const int c = c0 + (k * 32 + lane) * V;
+        if (c >= D) continue;
+        if constexpr (V >= 4) {
+#pragma unroll
+            for (int j = 0; j < V; j += 4) {
+                float4 v = make_float4(acc[k * V + j] * scale, acc[k * V + j + 1] * scale, acc[k * V + j + 2] * scale,
+                                       acc[k * V + j + 3] * scale);
+                float4* at = (float4*)(row + c + j);
+                if (add) {
+                    const float4 o = *at;
+                    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+                }
+                *at = v;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float v = acc[k * V + j] * scale;
+                row[c + j] = add ? row[c + j] + v : v;
+            }
+        }
+    }
+}
+
+template <int DT, int V>
+__global__ void __launch_bounds__(SUM_WARPS * 32)
+sum_runs_kernel(float* __restrict__ dtable, float* __restrict__ carry, const void* __restrict__ dout,
+                const int32_t* __restrict__ sorted_id, const int32_t* __restrict__ sorted_pos, int n, int vocab, int D,
+                int pieces, float scale, int accumulate) {
+    using TL = Tile<DT, V>;
+    using E = Elem<DT>;
+    const int lane = threadIdx.x & 31;
+    const int piece = blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
+    if (piece >= pieces) return;
+    const int c0 = blockIdx.y * TL::COLS;
+    const int i0 = piece * PIECE;
+    const int my = i0 + lane;
+    const int id = my < n ? sorted_id[my] : vocab;
+    const int pos = my < n ? sorted_pos[my] : 0;
+    const int prev = i0 > 0 ? sorted_id[i0 - 1] : -1;
+    const int next = i0 + PIECE < n ? sorted_id[i0 + PIECE] : vocab;
+    const int live = __popc(__ballot_sync(0xFFFFFFFFu, id < vocab));     // the tokens that count come first
+    if (live == 0) return;
+    // bit j: the run that item j belongs to ends with it, inside this piece
+    const int right = __shfl_down_sync(0xFFFFFFFFu, id, 1);
+    const uint32_t ends = __ballot_sync(0xFFFFFFFFu, lane == PIECE - 1 || right != id);
+    const char* base = (const char*)dout;
+    const size_t pitch = (size_t)D * E::SIZE;
+    float acc[TL::E];
+#pragma unroll
+    for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
+    bool head = __shfl_sync(0xFFFFFFFFu, id, 0) == prev;      // the first run began in an earlier piece
+    constexpr int AHEAD = 8;
+    for (int j0 = 0; j0 < live; j0 += AHEAD) {
+        Packet<DT, V> q[AHEAD][TL::NV];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int at = __shfl_sync(0xFFFFFFFFu, pos, j0 + a);
+            const char* row = base + (size_t)at * pitch;
+#pragma unroll
+            for (int k = 0; k < TL::NV; k++) {
+                const int c = c0 + (k * 32 + lane) * V;
+                if (j0 + a < live && c < D) q[a][k].load_stream(row + (size_t)c * E::SIZE);
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int j = j0 + a;
+            if (j >= live) break;
+#pragma unroll
+            for (int k = 0; k < TL::NV; k++) {
+                float f[V];
+                q[a][k].widen(f);
+#pragma unroll
+                for (int v = 0; v < V; v++) acc[k * V + v] += f[v];
+            }
+            if ((ends >> j) & 1u) {
+                const int run = __shfl_sync(0xFFFFFFFFu, id, j);
+                const bool tail = j == PIECE - 1 && run == next;
+                if (head || tail)
+                    put_row<DT, V>(carry + ((size_t)piece * 2 + (head ? 0 : 1)) * D, acc, c0, lane, D, 1.f, false);
+                else
+                    put_row<DT, V>(dtable + (size_t)run * D, acc, c0, lane, D, scale, accumulate);
+                head = false;
+#pragma unroll
+                for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
+            }
+        }
+    }
+}
+
+// One warp per piece in which a run begins that goes on: slot 1 of that piece, then slot 0 of every
+// piece that the run reaches.
+template <int V>
+__global__ void __launch_bounds__(SUM_WARPS * 32)
+join_runs_kernel(float* __restrict__ dtable, const float* __restrict__ carry, const int32_t* __restrict__ sorted_id,
+                 int n, int vocab, int D, int pieces, float scale, int accumulate) {
+    using TL = Tile<NVQ_F32, V>;
+    const int lane = threadIdx.x & 31;
+    const int piece = blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
+    if (piece + 1 >= pieces) return;
+    const int i0 = piece * PIECE, i1 = i0 + PIECE;      // i1 < n: another piece follows
+    const int id = sorted_id[i1 - 1];
+    if (id >= vocab || sorted_id[i1] != id) return;
+    if (sorted_id[i0] == id && i0 > 0 && sorted_id[i0 - 1] == id) return;     // began earlier
+    const int c0 = blockIdx.y * TL::COLS;
+    float acc[TL::E];
+    auto fetch = [&](const float* row, float* f) {
+#pragma unroll
+        for (int k = 0; k < TL::NV; k++) {
+            const int c = c0 + (k * 32 + lane) * V;
+            Packet<NVQ_F32, V> q;
+#pragma unroll
+            for (int w = 0; w < Packet<NVQ_F32, V>::WORDS; w++) q.w[w] = 0;
+            if (c < D) q.load(row + c);
+            q.widen(f + k * V);
+        }
+    };
+    fetch(carry + ((size_t)piece * 2 + 1) * D, acc);
+    // pieces piece + 1 ... : a piece belongs to the run while its first token has the run's id
+    for (int q0 = piece + 1; q0 < pieces; q0 += 32) {
+        const int mine = q0 + lane;
+        const bool in = mine < pieces && sorted_id[(size_t)mine * PIECE] == id;
+        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, in);
+        const int many = hit == 0xFFFFFFFFu ? 32 : __ffs(~hit) - 1;
+        constexpr int AHEAD = 8;
+        for (int a0 = 0; a0 < many; a0 += AHEAD) {
+            float f[AHEAD][TL::E];
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+                if (a0 + a < many) fetch(carry + (size_t)(q0 + a0 + a) * 2 * D, f[a]);
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+                if (a0 + a < many)
+#pragma unroll
+                    for (int e = 0; e < TL::E; e++) acc[e] += f[a][e];
+        }
+        if (many < 32) break;
+    }
+    put_row<NVQ_F32, V>(dtable + (size_t)id * D, acc, c0, lane, D, scale, accumulate);
+}
+
+size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+
+struct BwdSpace { size_t ids, pos, carry, total; };
+BwdSpace bwd_space(size_t T, size_t D) {
+    const size_t n = T < (size_t)SORT_MAX ? T : SORT_MAX;
+    BwdSpace s;
+    s.ids = align256(n * 4);
+    s.pos = align256(n * 4);
+    s.carry = align256((n + PIECE - 1) / PIECE * 2 * D * 4);
+    s.total = s.ids + s.pos + s.carry;
+    return s;
+}
+
+template <int DT>
+nvq_status sum_runs(float* dtable, float* carry, const char* dout, const int32_t* sid, const int32_t* spos, int n,
+                    int vocab, int D, float scale, int accumulate, cudaStream_t st) {
+    constexpr int V16 = 16 / Elem<DT>::SIZE, V4 = 4 / Elem<DT>::SIZE;
+    const int pieces = (n + PIECE - 1) / PIECE;
+    const bool wide = D % V16 == 0 && nvq_aligned(dout, 16) && nvq_aligned(dtable, 16);
+    const dim3 block(SUM_WARPS * 32);
+    auto grid = [&](int cols) { return dim3((pieces + SUM_WARPS - 1) / SUM_WARPS, (D + cols - 1) / cols); };
+    if (wide)
+        sum_runs_kernel<DT, V16><<<grid(Tile<DT, V16>::COLS), block, 0, st>>>(dtable, carry, dout, sid, spos, n, vocab,
+                                                                              D, pieces, scale, accumulate);
+    else if (V4 > 1 && D % V4 == 0 && nvq_aligned(dout, 4))
+        sum_runs_kernel<DT, V4><<<grid(Tile<DT, V4>::COLS), block, 0, st>>>(dtable, carry, dout, sid, spos, n, vocab,
+                                                                            D, pieces, scale, accumulate);
+    else
+        sum_runs_kernel<DT, 1><<<grid(Tile<DT, 1>::COLS), block, 0, st>>>(dtable, carry, dout, sid, spos, n, vocab, D,
+                                                                          pieces, scale, accumulate);
+    NVQ_LAUNCHED();
+    if (pieces > 1) {
+        if (D % 4 == 0 && nvq_aligned(dtable, 16))
+            join_runs_kernel<4><<<grid(Tile<NVQ_F32, 4>::COLS), block, 0, st>>>(dtable, carry, sid, n, vocab, D, pieces,
+                                                                                scale, accumulate);
+        else
+            join_runs_kernel<1><<<grid(Tile<NVQ_F32, 1>::COLS), block, 0, st>>>(dtable, carry, sid, n, vocab, D, pieces,
+                                                                                scale, accumulate);
+        NVQ_LAUNCHED();
+    }
+    return NVQ_OK;
+}
+
+}  // namespace
+
+extern "C" nvq_status nvq_embedding_fwd(void* d_out, const void* d_table, nvq_dtype dtype, const int32_t* d_ids,
+                                        size_t T, size_t V, size_t D, float scale, int device, void* stream) {
+    NVQ_REQUIRE(dtype == NVQ_F32 || dtype == NVQ_F16 || dtype == NVQ_BF16,
+                "nvq_embedding_fwd: table type %d; f32, f16 and bf16 are taken", (int)dtype);
+    NVQ_REQUIRE(V > 0 && V < (1u << 31) && D > 0 && D < (1u << 31) && T < ((size_t)1 << 31),
+                "nvq_embedding_fwd: V and D in [1, 2^31), T below 2^31");
+    if (T == 0) return NVQ_OK;
+    const size_t size = dtype == NVQ_F32 ? 4 : 2;
+    NVQ_REQUIRE(d_out && d_table && d_ids, "nvq_embedding_fwd: null buffer");
+    NVQ_REQUIRE(nvq_aligned(d_out, size) && nvq_aligned(d_table, size) && nvq_aligned(d_ids, 4),
+                "nvq_embedding_fwd: misaligned buffer");
+    nvq_status s = nvq_use_device(device);
+    if (s != NVQ_OK) return s;
+    int* status = nullptr;
+    s = nvq_status_word(device, &status);
+    if (s != NVQ_OK) return s;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == NVQ_F32) return lookup<NVQ_F32>(d_out, d_table, d_ids, T, V, D, scale, status, device, st);
+    if (dtype == NVQ_F16) return lookup<NVQ_F16>(d_out, d_table, d_ids, T, V, D, scale, status, device, st);
+    return lookup<NVQ_BF16>(d_out, d_table, d_ids, T, V, D, scale, status, device, st);
+}
+
+extern "C" nvq_status nvq_embedding_bwd_workspace_bytes(size_t T, size_t V, size_t D, size_t* bytes) {
+    NVQ_REQUIRE(bytes, "null out pointer");
+    (void)V;
+    *bytes = bwd_space(T, D).total;
+    return NVQ_OK;
+}
+
+extern "C" nvq_status nvq_embedding_bwd(float* d_dtable, const void* d_dout, nvq_dtype dout_dtype,
+                                        const int32_t* d_ids, size_t T, size_t V, size_t D, float scale,
+                                        int32_t padding_id, int accumulate, void* d_workspace, size_t workspace_bytes,
+                                        int device, void* stream) {
+    NVQ_REQUIRE(dout_dtype == NVQ_F32 || dout_dtype == NVQ_F16 || dout_dtype == NVQ_BF16,
+                "nvq_embedding_bwd: gradient type %d; f32, f16 and bf16 are taken", (int)dout_dtype);
+    NVQ_REQUIRE(V > 0 && V < (1u << 31) - 1 && D > 0 && D <= (1u << 22) && T < ((size_t)1 << 31),
+                "nvq_embedding_bwd: V in [1, 2^31 - 1), D in [1, 2^22], T below 2^31");
+    const size_t size = dout_dtype == NVQ_F32 ? 4 : 2;
+    NVQ_REQUIRE(d_dtable && nvq_aligned(d_dtable, 4), "nvq_embedding_bwd: null or misaligned table gradient");
+    NVQ_REQUIRE(T == 0 || (d_dout && d_ids && nvq_aligned(d_dout, size) && nvq_aligned(d_ids, 4)),
+                "nvq_embedding_bwd: null or misaligned buffer");
+    const BwdSpace sp = bwd_space(T, D);
+    NVQ_REQUIRE(T == 0 || (d_workspace && workspace_bytes >= sp.total && nvq_aligned(d_workspace, 256)),
+                "nvq_embedding_bwd: workspace of %zu bytes (256-byte aligned) required", sp.total);
+    nvq_status s = nvq_use_device(device);
+    if (s != NVQ_OK) return s;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T == 0) {
+        if (!accumulate) NVQ_CUDA(cudaMemsetAsync(d_dtable, 0, V * D * sizeof(float), st));
+        return NVQ_OK;
+    }
+    int* status = nullptr;
+    s = nvq_status_word(device, &status);
+    if (s != NVQ_OK) return s;
+    static std::atomic<bool> attr_set[64];   // per device; setting the attribute twice is harmless
+    if (!attr_set[device]) {
+        NVQ_CUDA(cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)sizeof(SortShared)));
+        attr_set[device] = true;
+    }
+    int32_t* sid = (int32_t*)d_workspace;
+    int32_t* spos = (int32_t*)((char*)d_workspace + sp.ids);
+    float* carry = (float*)((char*)d_workspace + sp.ids + sp.pos);
+    int value_bits = 1;
+    while (((size_t)1 << value_bits) <= V) value_bits++;      // V itself marks a token that takes no part
+    // more tokens than one cluster sorts: one part after the other, each adding to the table
+    for (size_t t0 = 0; t0 < T; t0 += SORT_MAX) {
+        const int n = (int)(T - t0 < (size_t)SORT_MAX ? T - t0 : SORT_MAX);
+        const int add = accumulate || t0 > 0;
+        SortParams q;
+        q.ids = d_ids + t0;
+        q.sorted_id = sid;
+        q.sorted_pos = spos;
+        q.n = n;
+        q.vocab = (int)V;
+        q.padding_id = padding_id;
+        q.passes = (value_bits + MAX_BITS - 1) / MAX_BITS;
+        q.bits = (value_bits + q.passes - 1) / q.passes;
+        q.clear = add ? nullptr : d_dtable;
+        q.clear_floats = add ? 0 : V * D;
+        q.status = status;
+        const int ctas = n <= SORT_THREADS ? 1 : MAX_CLUSTER;
+        q.chunk_log2 = 5;
+        while (((size_t)ctas << q.chunk_log2) < (size_t)n) q.chunk_log2++;
+        // enough further clusters to clear the table with about every SM, none for a small one
+        size_t clearing = (q.clear_floats + 32767) / 32768;
+        const size_t most = nvq_sm_count(device) - ctas;
+        if (clearing > most) clearing = most;
+        clearing = (clearing + ctas - 1) / ctas * ctas;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(ctas + clearing));
+        cfg.blockDim = dim3(SORT_THREADS);
+        cfg.dynamicSmemBytes = sizeof(SortShared);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ctas;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        NVQ_CUDA(cudaLaunchKernelEx(&cfg, sort_tokens_kernel, q));
+        NVQ_LAUNCHED();
+        const char* part = (const char*)d_dout + t0 * D * size;
+        if (dout_dtype == NVQ_F32)
+            s = sum_runs<NVQ_F32>(d_dtable, carry, part, sid, spos, n, (int)V, (int)D, scale, add, st);
+        else if (dout_dtype == NVQ_F16)
+            s = sum_runs<NVQ_F16>(d_dtable, carry, part, sid, spos, n, (int)V, (int)D, scale, add, st);
+        else
+            s = sum_runs<NVQ_BF16>(d_dtable, carry, part, sid, spos, n, (int)V, (int)D, scale, add, st);
+        if (s != NVQ_OK) return s;
+    }
+    return NVQ_OK;
+}

@@ -145,6 +145,23 @@ class DeviceBuffer:
             pass
 
 
+class DeviceView:
+    """Device memory owned by someone else, with ``DeviceBuffer``'s addressing."""
+
+    def __init__(self, ptr: int, nbytes: int, device: int = 0):
+        self.ptr, self.nbytes, self.device = ptr, nbytes, device
+
+    def at(self, offset: int) -> C.c_void_p:
+        return C.c_void_p(self.ptr + offset)
+
+    def to_numpy(self, dtype, shape) -> np.ndarray:
+        out = np.empty(shape, dtype)
+        check(lib().nvq_memcpy_d2h(out.ctypes.data_as(C.c_void_p), C.c_void_p(self.ptr), out.nbytes,
+                                   self.device, None))
+        check(lib().nvq_device_sync(self.device))
+        return out
+
+
 class _Pinned:
     def __init__(self, nbytes: int):
         p = C.c_void_p()

@@ -561,3 +561,168 @@ def dropout_host(x, mask, keep_prob: float, device: int = 0):
     o = DeviceBuffer(max(4, x.nbytes), device)
     check(lib().nvq_dropout_f32(o.at(0), dx.at(0), dm.at(0), x.size, C.c_float(keep_prob), device, None))
     return o.to_numpy(np.float32, x.shape)
+
+
+# ------------------------------------------------------------------ embedding
+_FLOATS = {"f32": 4, "f16": 2, "bf16": 2}
+_HOST_FLOATS = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.uint16): "bf16"}
+
+
+def _float_type(name: str, allowed=_FLOATS) -> int:
+    if name not in allowed:
+        raise ValueError(f"dtype must be one of {tuple(allowed)}, not {name!r}")
+    return allowed[name]
+
+
+def _holds(what: str, buf, nbytes: int) -> None:
+    if buf is None or buf.nbytes < nbytes:
+        raise ValueError(f"{what} must hold {nbytes} bytes, got {None if buf is None else buf.nbytes}")
+
+
+def embedding_device(out: DeviceBuffer, table: DeviceBuffer, dtype: str, ids: DeviceBuffer, t: int, v: int, d: int,
+                     scale: float = 1.0, stream=None) -> None:
+    """out (t, d) = scale * table (v, d)[ids], in the table's type ("f32", "f16" or "bf16"); ids
+    int32.  An id outside [0, v) gives a row of zeros and is reported by ``check_device_errors``."""
+    size = _float_type(dtype)
+    _holds("out", out, t * d * size)
+    _holds("table", table, v * d * size)
+    _holds("ids", ids, t * 4)
+    check(lib().nvq_embedding_fwd(out.at(0), table.at(0), _lib.DTYPE_IDS[dtype], ids.at(0), t, v, d,
+                                  C.c_float(scale), table.device, _sptr(stream)))
+
+
+def embedding_bwd_workspace_bytes(t: int, v: int, d: int) -> int:
+    out = C.c_size_t()
+    check(lib().nvq_embedding_bwd_workspace_bytes(t, v, d, C.byref(out)))
+    return out.value
+
+
+def embedding_bwd_device(dtable: DeviceBuffer, dout: DeviceBuffer, dtype: str, ids: DeviceBuffer, t: int, v: int,
+                         d: int, workspace: DeviceBuffer, scale: float = 1.0, padding_id: int | None = None,
+                         accumulate: bool = False, stream=None) -> None:
+    """dtable (v, d) fp32 = scale * the sums of dout's rows (t, d; ``dtype``) per id, or that added to
+    what dtable holds with ``accumulate`` (a table tied to the output projection).  Tokens whose id is
+    ``padding_id`` take no part.  The sums are added in the tokens' order: equal inputs, equal bits."""
+    size = _float_type(dtype)
+    _holds("dtable", dtable, v * d * 4)
+    _holds("dout", dout, t * d * size)
+    _holds("ids", ids, t * 4)
+    check(lib().nvq_embedding_bwd(dtable.at(0), dout.at(0), _lib.DTYPE_IDS[dtype], ids.at(0), t, v, d,
+                                  C.c_float(scale), -1 if padding_id is None else padding_id, int(accumulate),
+                                  workspace.at(0), workspace.nbytes, dtable.device, _sptr(stream)))
+
+
+def _host_ids(ids, v: int) -> np.ndarray:
+    ids = np.asarray(ids)
+    if ids.dtype.kind not in "iu":
+        raise TypeError(f"ids must be integers, got {ids.dtype}")
+    if ids.size and (int(ids.min()) < 0 or int(ids.max()) >= v):
+        raise IndexError(f"id out of range for {v} rows")
+    return np.ascontiguousarray(ids, np.int32)
+
+
+def _host_float(a) -> tuple[np.ndarray, str]:
+    a = np.ascontiguousarray(a)
+    if a.dtype not in _HOST_FLOATS:
+        raise TypeError(f"float32, float16 or uint16 (bf16 bits) expected, got {a.dtype}")
+    return a, _HOST_FLOATS[a.dtype]
+
+
+def embedding_host(table, ids, scale: float = 1.0, device: int = 0) -> np.ndarray:
+    """scale * table[ids] for host arrays: ``table`` (V, D) float32, float16 or bf16 bits (uint16),
+    ``ids`` integers of any shape; returns ids.shape + (D,) in the table's type."""
+    table, dtype = _host_float(table)
+    v, d = table.shape
+    ids = _host_ids(ids, v)
+    if ids.size == 0 or d == 0:
+        return np.empty(ids.shape + (d,), table.dtype)
+    dt, di = DeviceBuffer.from_numpy(table, device), DeviceBuffer.from_numpy(ids, device)
+    do = DeviceBuffer(ids.size * d * table.itemsize, device)
+    embedding_device(do, dt, dtype, di, ids.size, v, d, scale)
+    return do.to_numpy(table.dtype, ids.shape + (d,))
+
+
+def embedding_bwd_host(dout, ids, v: int, scale: float = 1.0, padding_id: int | None = None,
+                       device: int = 0) -> np.ndarray:
+    """Gradient of ``embedding_host``'s table: (v, D) float32 from dout (ids.shape + (D,))."""
+    dout, dtype = _host_float(dout)
+    ids = _host_ids(ids, v)
+    d = dout.shape[-1]
+    if dout.shape != ids.shape + (d,):
+        raise ValueError(f"gradient of shape {dout.shape} for ids of shape {ids.shape}")
+    if d == 0:
+        return np.zeros((v, 0), np.float32)
+    t = ids.size
+    dg, di = DeviceBuffer.from_numpy(dout, device), DeviceBuffer.from_numpy(ids, device)
+    o, ws = DeviceBuffer(v * d * 4, device), DeviceBuffer(embedding_bwd_workspace_bytes(t, v, d), device)
+    embedding_bwd_device(o, dg, dtype, di, t, v, d, ws, scale, padding_id)
+    return o.to_numpy(np.float32, (v, d))
+
+
+# ------------------------------------------------------------------ gradient norm and clipping
+_GRADS = {**_FLOATS, "f64": 8}
+
+
+def grad_norm_workspace_bytes() -> int:
+    out = C.c_size_t()
+    check(lib().nvq_grad_norm_workspace_bytes(C.byref(out)))
+    return out.value
+
+
+def _tensor_list(what: str, bufs, counts, dtypes):
+    n = len(bufs)
+    if len(counts) != n or (not isinstance(dtypes, str) and len(dtypes) != n):
+        raise ValueError("tensors, counts and dtypes must be of one length")
+    names = [dtypes] * n if isinstance(dtypes, str) else dtypes
+    sizes = [_float_type(name, _GRADS) for name in names]
+    ptrs = []
+    for b, count, size in zip(bufs, counts, sizes):
+        if count < 0 or b.nbytes < count * size:
+            raise ValueError(f"{what}: a buffer of {b.nbytes} bytes does not hold {count} elements")
+        ptrs.append(b.ptr)
+    if len(set(ptrs)) != n and len({p for p, c in zip(ptrs, counts) if c}) != sum(1 for c in counts if c):
+        raise ValueError(f"{what}: a tensor is listed twice")
+    return ((C.c_void_p * n)(*ptrs), (C.c_size_t * n)(*counts),
+            (C.c_int32 * n)(*[_lib.DTYPE_IDS[name] for name in names]), n)
+
+
+def grad_norm_device(norm: DeviceBuffer, grads, counts, dtypes, workspace: DeviceBuffer,
+                     max_norm: float = float("inf"), stream=None) -> None:
+    """norm (2 floats) = the 2-norm of all ``grads`` together, and the factor that clipping to
+    ``max_norm`` would apply.  ``grads``: device buffers, ``counts``: their elements, ``dtypes``: one
+    name for all or one each ("f32", "f16", "bf16", "f64")."""
+    _holds("norm", norm, 8)
+    ptrs, n_el, types, n = _tensor_list("grads", grads, counts, dtypes)
+    check(lib().nvq_grad_norm(norm.at(0), ptrs, n_el, types, n, float(max_norm), workspace.at(0), workspace.nbytes,
+                              norm.device, _sptr(stream)))
+
+
+def clip_grads_device(norm: DeviceBuffer, grads, counts, dtypes, max_norm: float, workspace: DeviceBuffer, out=None,
+                      stream=None) -> None:
+    """``grad_norm_device``, then every gradient times the factor: in place, or into ``out``."""
+    _holds("norm", norm, 8)
+    ptrs, n_el, types, n = _tensor_list("grads", grads, counts, dtypes)
+    to = None if out is None else _tensor_list("out", out, counts, dtypes)[0]
+    check(lib().nvq_clip_grads(norm.at(0), to, ptrs, n_el, types, n, float(max_norm), workspace.at(0),
+                               workspace.nbytes, norm.device, _sptr(stream)))
+
+
+def clip_grad_norm(parameters, max_norm: float, device: int = 0) -> np.float32:
+    """Scales the gradients of ``parameters`` (anything with ``.grad``; None is skipped, a parameter
+    listed twice counts once) in place so that their joint 2-norm is at most ``max_norm``; returns
+    the norm before.  float32, float64 and float16 gradients."""
+    if not max_norm > 0:
+        raise ValueError(f"max_norm must be above 0, got {max_norm}")
+    params = [p for p in {id(p): p for p in parameters}.values() if p.grad is not None and p.grad.size]
+    kinds = {np.dtype(np.float32): "f32", np.dtype(np.float64): "f64", np.dtype(np.float16): "f16"}
+    for p in params:
+        if p.grad.dtype not in kinds:
+            raise TypeError(f"gradient must be float32, float64 or float16, got {p.grad.dtype}")
+    bufs = [DeviceBuffer.from_numpy(p.grad, device) for p in params]
+    norm, ws = DeviceBuffer(8, device), DeviceBuffer(grad_norm_workspace_bytes(), device)
+    clip_grads_device(norm, bufs, [p.grad.size for p in params], [kinds[p.grad.dtype] for p in params], max_norm, ws)
+    value, coef = norm.to_numpy(np.float32, (2,))
+    if coef != 1.0:
+        for p, b in zip(params, bufs):
+            p.grad[...] = b.to_numpy(p.grad.dtype, p.grad.shape)
+    return value

@@ -486,3 +486,43 @@ class Dropout(Layer):
 
     def __repr__(self):
         return f"Dropout(p={self.p})"
+
+
+class Embedding(Layer):
+    """Rows of a (num_embeddings, embedding_dim) table by integer id, times ``scale``: ids of any shape
+    in, ids.shape + (embedding_dim,) float32 out.  ``backward`` assigns the table's gradient (tokens
+    whose id is ``padding_id`` take no part) and returns None, since ids have no gradient."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_id: int | None = None,
+                 init=None, device: int = 0) -> None:
+        super().__init__()
+        if padding_id is not None and not 0 <= padding_id < num_embeddings:
+            raise ValueError(f"padding_id {padding_id} is not an id of {num_embeddings} rows")
+        self.num_embeddings, self.embedding_dim = int(num_embeddings), int(embedding_dim)
+        self.scale, self.padding_id = float(scale), padding_id
+        self.init_fn = init
+        self.device = device
+        self.weight = None
+        self._ids = None
+        self.reset_parameters()
+
+    def reset_parameters(self, initializer=None) -> None:
+        init = initializer or self.init_fn or small_normal
+        self.weight = Parameters(np.asarray(init((self.num_embeddings, self.embedding_dim)), dtype=np.float32))
+        self.weight.name = "embedding weight"
+
+    def forward(self, ids: np.ndarray) -> np.ndarray:
+        self._ids = np.asarray(ids)
+        return F.embedding_host(self.weight.data, self._ids, self.scale, self.device)
+
+    def backward(self, grad: np.ndarray) -> None:
+        if self._ids is None:
+            raise RuntimeError("forward must be called before backward")
+        self.weight.grad = F.embedding_bwd_host(_as_f32(grad, self.device), self._ids, self.num_embeddings,
+                                                self.scale, self.padding_id, self.device)
+
+    def parameters(self):
+        return [self.weight]
+
+    def __repr__(self):
+        return f"Embedding(num_embeddings={self.num_embeddings}, embedding_dim={self.embedding_dim}, scale={self.scale})"

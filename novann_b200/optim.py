@@ -1,6 +1,7 @@
-"""Vanilla ``SGD`` with the reference's contract (``novann/optim/sgd.py:6-87``, the path with
-momentum 0, weight decay 0 and no clipping): ``p.data -= lr * p.grad`` on the GPU, written
-back into the same NumPy arrays so the layers' ``Parameters`` stay the source of truth."""
+"""``SGD`` with the reference's contract (``novann/optim/sgd.py:6-87``, the path with momentum 0 and
+weight decay 0): with ``max_grad_norm`` the gradients are first scaled in place to that joint norm at
+most, then ``p.data -= lr * p.grad`` on the GPU, written back into the same NumPy arrays so the
+layers' ``Parameters`` stay the source of truth."""
 from __future__ import annotations
 
 import ctypes as C
@@ -14,14 +15,19 @@ from .device import DeviceBuffer
 class SGD:
     def __init__(self, parameters, lr: float, momentum: float = 0, weight_decay: float = 0,
                  max_grad_norm=None, device: int = 0) -> None:
-        if momentum or weight_decay or max_grad_norm:
-            raise NotImplementedError("only the vanilla SGD path (momentum 0, weight decay 0, "
-                                      "no clipping) is built")
+        if momentum or weight_decay:
+            raise NotImplementedError("only the SGD path with momentum 0 and weight decay 0 is built")
+        if max_grad_norm and not max_grad_norm > 0:
+            raise ValueError(f"max_grad_norm must be above 0, got {max_grad_norm}")
+        self.max_grad_norm = max_grad_norm or None
         self.params = list(parameters)
         self.lr = float(lr)
         self.device = device
 
     def step(self) -> None:
+        if self.max_grad_norm is not None:
+            from .functional import clip_grad_norm
+            clip_grad_norm(self.params, self.max_grad_norm, self.device)
         for p in self.params:
             if p.grad is None:
                 continue

@@ -17,7 +17,7 @@ import ctypes as C
 import numpy as np
 
 from ._lib import check, lib
-from .device import DeviceBuffer, Event, Stream, _sptr
+from .device import DeviceBuffer, DeviceView, Event, Stream, _sptr
 
 
 def shard_rows(n_rows: int, rank: int, world: int) -> tuple[int, int]:
@@ -83,23 +83,6 @@ class Communicator:
             self.handle = None
 
 
-class _DeviceView:
-    """Device memory owned by someone else, with ``DeviceBuffer``'s addressing."""
-
-    def __init__(self, ptr: int, nbytes: int, device: int):
-        self.ptr, self.nbytes, self.device = ptr, nbytes, device
-
-    def at(self, offset: int) -> C.c_void_p:
-        return C.c_void_p(self.ptr + offset)
-
-    def to_numpy(self, dtype, shape) -> np.ndarray:
-        out = np.empty(shape, dtype)
-        check(lib().nvq_memcpy_d2h(out.ctypes.data_as(C.c_void_p), C.c_void_p(self.ptr), out.nbytes,
-                                   self.device, None))
-        check(lib().nvq_device_sync(self.device))
-        return out
-
-
 class PeerGroup:
     """Gradient all-reduce fused with the SGD update over NVLink peer memory (``nvq_peer_*``):
     one kernel per step and rank instead of an NCCL all-reduce plus the SGD kernel.
@@ -134,9 +117,9 @@ class PeerGroup:
         for parity in (0, 1):
             p = C.c_void_p()
             check(lib().nvq_peer_grad_buffer(C.c_void_p(self.handle), parity, C.byref(p)))
-            self.grad_views.append(_DeviceView(p.value, self.n * 4, device))
+            self.grad_views.append(DeviceView(p.value, self.n * 4, device))
 
-    def grads(self) -> _DeviceView:
+    def grads(self) -> DeviceView:
         """Where the backward pass of the NEXT step writes this rank's gradients."""
         return self.grad_views[self.calls & 1]
 
@@ -167,10 +150,17 @@ class MLPTrainStep:
     """``step(x, labels)`` runs one training step on the device and returns nothing; read
     results with ``logits()``, ``loss()``, ``grads()``, ``params()``.  Data parallel: ``comm=``
     (NCCL all-reduce, then the SGD kernel) or ``peer=`` (``PeerGroup``: all-reduce and update in
-    one kernel over NVLink peer memory)."""
+    one kernel over NVLink peer memory).  ``max_grad_norm`` clips the (all-reduced, averaged)
+    gradient before the update; ``grad_norm()`` then gives its norm before the cut."""
 
     def __init__(self, params, batch: int, lr: float, device: int = 0, comm: Communicator | None = None,
-                 gate=None, collective_timeout_ms: int = 30000, peer: PeerGroup | None = None):
+                 gate=None, collective_timeout_ms: int = 30000, peer: PeerGroup | None = None,
+                 max_grad_norm: float | None = None):
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f"max_grad_norm must be above 0, got {max_grad_norm}")
+        if max_grad_norm is not None and peer is not None:
+            raise ValueError("the peer group's kernel updates as it reduces: it cannot clip in between")
+        self.max_grad_norm = max_grad_norm
         self.dims = [params[0].shape[1]] + [params[2 * i].shape[0] for i in range(len(params) // 2)]
         self.nl = len(self.dims) - 1
         self.batch, self.lr, self.device, self.comm = batch, float(lr), device, comm
@@ -203,6 +193,12 @@ class MLPTrainStep:
         self.d_g = [DeviceBuffer(f4 * d, device) for d in self.dims]     # gradient w.r.t. each activation
         self.d_yhat = DeviceBuffer(f4 * self.dims[-1], device)
         self.d_loss = DeviceBuffer(4, device)
+        self.d_norm = self.d_norm_ws = None
+        self._norm_scale = 1.0
+        if max_grad_norm is not None:
+            from .functional import grad_norm_workspace_bytes
+            self.d_norm = DeviceBuffer(8, device)
+            self.d_norm_ws = DeviceBuffer(grad_norm_workspace_bytes(), device)
         self.ev_fork = [Event(device) for _ in range(self.nl)]
         self.ev_join = Event(device)
         self.ev_loss = Event(device)
@@ -271,6 +267,12 @@ class MLPTrainStep:
         if self.comm is not None and self.comm.world > 1:
             self.comm.allreduce_sum(self.d_grads, self.n_params, stream=self.stream)
             scale = 1.0 / self.comm.world
+        if self.max_grad_norm is not None:
+            # d_grads holds 1 / scale times the averaged gradient: the limit is scaled alike
+            from .functional import clip_grads_device
+            clip_grads_device(self.d_norm, [self.d_grads], [self.n_params], "f32", self.max_grad_norm / scale,
+                              self.d_norm_ws, stream=self.stream)
+            self._norm_scale = scale
         check(L.nvq_sgd_step_f32(self.d_params.at(0), self.d_grads.at(0), self.n_params,
                                  C.c_float(self.lr), C.c_float(scale), dev, st))
 
@@ -324,8 +326,8 @@ class MLPTrainStep:
 
     def kernels_per_step(self) -> int:
         """Kernel launches of this library in one step: nl forward, 1 loss, per layer one GEMM for
-        dW with db as its by-product (+ one for dX except for the first layer), 1 SGD."""
-        return self.nl + 1 + (2 * self.nl - 1) + 1
+        dW with db as its by-product (+ one for dX except for the first layer), 2 for clipping, 1 SGD."""
+        return self.nl + 1 + (2 * self.nl - 1) + (2 if self.max_grad_norm is not None else 0) + 1
 
     def step(self, x: np.ndarray, labels: np.ndarray) -> None:
         if self.gate is not None:
@@ -356,6 +358,12 @@ class MLPTrainStep:
 
     def loss(self) -> np.float32:
         return self.d_loss.to_numpy(np.float32, (1,))[0]
+
+    def grad_norm(self) -> np.float32:
+        """Norm of the last step's averaged gradient before it was cut (with ``max_grad_norm``)."""
+        if self.d_norm is None:
+            raise RuntimeError("the step was made without max_grad_norm")
+        return np.float32(self.d_norm.to_numpy(np.float32, (2,))[0] * self._norm_scale)
 
     def grads(self) -> list[np.ndarray]:
         return unflatten_params(self.d_grads.to_numpy(np.float32, (self.n_params,)), self.dims)
