@@ -228,16 +228,16 @@ def _run_own(s):
         bias = None if s["bias"] is None else _view(s["bias"])
         space = _view(_hold := _space(F.linear_ce_workspace_bytes(m, v, k, backward=back)))
         head = torch.empty(2, device="cuda")
-        lse, rows = torch.empty(m, device="cuda"), torch.empty(m, device="cuda")
+        stats, rows = torch.empty(2, m, device="cuda"), torch.empty(m, device="cuda")
         x, w, labels = _view(s["x"]), _view(s["w"]), _view(s["labels"])
-        F.linear_ce_device(_view(head), _view(lse), x, w, dtype, labels, m, v, k, space, bias=bias,
+        F.linear_ce_device(_view(head), _view(stats), x, w, dtype, labels, m, v, k, space, bias=bias,
                            row_loss=_view(rows), stream=stream)
         out = {"loss": head[0], "rows": rows}
         if back:
             out["dx"], out["dw"] = torch.empty_like(s["x"]), torch.empty_like(s["w"])
             if bias is not None:
                 out["db"] = torch.empty(v, device="cuda")
-            F.linear_ce_bwd_device(_view(out["dx"]), _view(out["dw"]), x, w, dtype, labels, _view(lse), _view(head),
+            F.linear_ce_bwd_device(_view(out["dx"]), _view(out["dw"]), x, w, dtype, labels, _view(stats), _view(head),
                                    m, v, k, space, bias=bias, db=None if bias is None else _view(out["db"]),
                                    grad_dtype=dtype, grad_scale=s["loss_scale"], stream=stream)
         return out
