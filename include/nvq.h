@@ -393,6 +393,40 @@ nvq_status nvq_embedding_bwd(float* d_dtable, const void* d_dout, nvq_dtype dout
                              size_t T, size_t V, size_t D, float scale, int32_t padding_id, int accumulate,
                              void* d_workspace, size_t workspace_bytes, int device, void* stream);
 
+/* ---------------------------------------------------------------- linear + softmax cross entropy
+ * The last layer of a classifier over a large vocabulary and its loss in one: X (M x K) and W (V x K) f16 or
+ * bf16 (one type, 16-byte aligned rows: K % 8 == 0), bias V fp32 or NULL, labels M int32.  M, V any.
+ *   l = X W^T + b (fp32);  lse_m = log sum_v exp l_mv;  loss_m = lse_m - l_m,label(m)
+ * The M x V logits are never kept.  A row whose label is ignore_index counts for nothing; a label outside
+ * [0, V) that is not ignore_index is treated alike and reported by nvq_device_error_flag (code 85).  This is
+ * the ordinary log-likelihood; nvq_softmax_ce_f32 is the reference's loss (softmax applied twice).
+ *   d_loss_count[0] = sum of the rows' losses, or their mean over the rows that count (0 without any)
+ *   d_loss_count[1] = number of rows that count;  d_row_loss (M fp32, may be NULL)
+ *   d_row_stats (2 M fp32): the rows' largest logits, then log sum_v exp(l - largest); their sums are lse
+ * A bias of -inf takes its entry out of the vocabulary; a row with nothing left has an infinite loss and no
+ * gradient.
+ */
+enum { NVQ_REDUCE_SUM = 0, NVQ_REDUCE_MEAN = 1 };
+/* 256-byte aligned; backward != 0: enough for nvq_linear_ce_bwd too (a piece of at most max(64 Mi, 8192 M)
+ * values of the logits' gradient in 16 bits, and an fp32 dX where there are several pieces).  Contents need not
+ * be kept or cleared between calls. */
+nvq_status nvq_linear_ce_workspace_bytes(size_t M, size_t V, size_t K, int backward, size_t* bytes);
+nvq_status nvq_linear_ce_fwd(float* d_loss_count, float* d_row_loss, float* d_row_stats, const void* d_x, const void* d_w,
+                             nvq_dtype dtype, const float* d_bias, const int32_t* d_labels, size_t M, size_t V,
+                             size_t K, int32_t ignore_index, int reduction, void* d_workspace,
+                             size_t workspace_bytes, int device, void* stream);
+/* Gradients of grad_scale * loss from what nvq_linear_ce_fwd left in d_row_stats and d_loss_count, the logits computed
+ * again: with g = s (softmax(l) - onehot), s = grad_scale (over the count for the mean),
+ *   dX (M x K) = g W;  dW (V x K) = g^T X;  db (V fp32) = column sums of g
+ * Any of them may be NULL.  dX and dW are fp32 or of the operands' type (16-byte aligned).  The tensor cores
+ * read g rounded to the operands' type (2^-8 of a value for bf16, 2^-11 for f16), sums are fp32; db is summed
+ * from fp32 values.  Every sum has a fixed order.  Rows that do not count give a dX of 0. */
+nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_dtype, float* d_db, const void* d_x,
+                             const void* d_w, nvq_dtype dtype, const float* d_bias, const int32_t* d_labels,
+                             const float* d_row_stats, const float* d_loss_count, float grad_scale, size_t M, size_t V,
+                             size_t K, int32_t ignore_index, int reduction, void* d_workspace,
+                             size_t workspace_bytes, int device, void* stream);
+
 /* ---------------------------------------------------------------- gradient norm and clipping
  * The clipping of SGD (novann/optim/sgd.py:6-87) for any list of tensors.  h_grads, h_counts (elements) and
  * h_dtypes (nvq_dtype: f32, f16, bf16 or f64, mixed freely) are host arrays of n_tensors entries, read before

@@ -9,7 +9,7 @@ reshape.)"""
 from . import functional, quant  # noqa: F401
 from .layers import (BatchNorm1d, BatchNorm2d, Conv2d, Dropout, Embedding, Flatten, GlobalAvgPool2d,  # noqa: F401
                      Linear, MaxPool2d, QuantConv2d, QuantLinear, ReLU)
-from .losses import CrossEntropyLoss  # noqa: F401
+from .losses import CrossEntropyLoss, LinearCrossEntropyLoss  # noqa: F401
 from .model import Sequential  # noqa: F401
 from .module import Layer, Module, Parameters  # noqa: F401
 from .optim import SGD, AdamW  # noqa: F401
@@ -20,5 +20,5 @@ register_if_imported()
 __all__ = ["functional", "quant", "Linear", "QuantLinear", "ReLU", "Conv2d", "QuantConv2d",
            "BatchNorm1d", "BatchNorm2d", "MaxPool2d", "GlobalAvgPool2d", "Flatten", "Dropout",
            "Embedding",
-           "Sequential", "CrossEntropyLoss", "SGD", "AdamW", "Layer", "Module", "Parameters",
+           "Sequential", "CrossEntropyLoss", "LinearCrossEntropyLoss", "SGD", "AdamW", "Layer", "Module", "Parameters",
            "register_with_novann"]

@@ -24,6 +24,8 @@ LINEAR_CODES_FINITE = 32
 CONV_AUTO, CONV_PATCH_MATRIX, CONV_CTA_PAIR = 0, 1, 2
 PAD_MODES = {"zeros": 0, "reflect": 1, "replicate": 2, "circular": 3}
 
+REDUCTIONS = {"sum": 0, "mean": 1}
+
 OK, ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT, ERR_NCCL = 0, -1, -2, -3, -4, -5
 
 vp, sz, i32, f32c, u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_uint64
@@ -102,6 +104,10 @@ SIGNATURES = {
     "nvq_embedding_fwd": (i32, [vp, vp, i32, vp, sz, sz, sz, f32c, i32, vp]),
     "nvq_embedding_bwd_workspace_bytes": (i32, [sz, sz, sz, C.POINTER(sz)]),
     "nvq_embedding_bwd": (i32, [vp, vp, i32, vp, sz, sz, sz, f32c, C.c_int32, i32, vp, sz, i32, vp]),
+    "nvq_linear_ce_workspace_bytes": (i32, [sz, sz, sz, i32, C.POINTER(sz)]),
+    "nvq_linear_ce_fwd": (i32, [vp, vp, vp, vp, vp, i32, vp, vp, sz, sz, sz, C.c_int32, i32, vp, sz, i32, vp]),
+    "nvq_linear_ce_bwd": (i32, [vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, vp, f32c, sz, sz, sz, C.c_int32, i32, vp, sz,
+                                i32, vp]),
     "nvq_grad_norm_workspace_bytes": (i32, [C.POINTER(sz)]),
     "nvq_grad_norm": (i32, [vp, vp, vp, vp, sz, f64c, vp, sz, i32, vp]),
     "nvq_clip_grads": (i32, [vp, vp, vp, vp, vp, sz, f64c, vp, sz, i32, vp]),

@@ -139,9 +139,11 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
     if (blockIdx.x >= ctas) {               // not the sorting cluster: clear the table
         const size_t first = (size_t)(blockIdx.x - ctas) * SORT_THREADS + tid;
         const size_t step = (size_t)(gridDim.x - ctas) * SORT_THREADS;
-        const size_t quads = ((uintptr_t)p.clear & 15) == 0 ? p.clear_floats / 4 : 0;
-        for (size_t i = first; i < quads; i += step) stg_stream_128(p.clear + 4 * i, make_uint4(0, 0, 0, 0));
-        for (size_t i = quads * 4 + first; i < p.clear_floats; i += step) p.clear[i] = 0.f;
+        const size_t octs = ((uintptr_t)p.clear & 31) == 0 ? p.clear_floats / 8 : 0;
+        const u32x8 zero = {};
+#pragma unroll 4
+        for (size_t i = first; i < octs; i += step) stg_stream_256(p.clear + 8 * i, zero);
+        for (size_t i = octs * 8 + first; i < p.clear_floats; i += step) p.clear[i] = 0.f;
         return;
     }
 
@@ -149,8 +151,9 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
     const int lo = (int)rank << p.chunk_log2;
     const int count = max(0, min(chunk, p.n - lo));
     const int bins = 1 << p.bits;
-    // warp w owns items [w * 32 * ITEMS, ...) of the CTA's run, in rounds of 32
-    const int w0 = warp * 32 * ITEMS;
+    // warp w owns items [w * 32 * rounds, ...) of the CTA's run, in rounds of 32
+    const int rounds = max(1, chunk / SORT_THREADS);
+    const int w0 = warp * 32 * rounds;
     uint32_t key[ITEMS], pos[ITEMS];
     for (int pass = 0; pass < p.passes; pass++) {
         const int shift = pass * p.bits;
@@ -159,6 +162,7 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
         uint32_t before[ITEMS / 2];         // 16-bit ranks within the warp's run, packed in pairs
 #pragma unroll
         for (int r = 0; r < ITEMS; r++) {
+            if (r >= rounds) break;
             const int i = w0 + r * 32 + lane;
             const bool live = i < count;
             key[r] = 0;
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
 #pragma unroll
         for (int r = 0; r < ITEMS; r++) {
             const int i = w0 + r * 32 + lane;
-            if (i >= count) continue;
+            if (r >= rounds || i >= count) break;
             const uint32_t d = (key[r] >> shift) & (bins - 1);
             const uint32_t rk = (r & 1) ? before[r >> 1] >> 16 : before[r >> 1] & 0xFFFFu;
             const uint32_t to = sh.base[d] + sh.hist[warp][d] + rk;
@@ -355,22 +359,21 @@ sum_runs_kernel(float* __restrict__ dtable, float* __restrict__ carry, const voi
     }
 }
 
-// One warp per piece in which a run begins that goes on: slot 1 of that piece, then slot 0 of every
-// piece that the run reaches.
+// The runs that cross pieces: slot 1 of the piece where one begins, then slot 0 of every piece that it
+// reaches.  A warp looks at one piece and adds up a run of at most LONG_RUN pieces by itself; a longer one
+// (a frequent token: one in sixteen tokens of a 65536-token batch makes 128 pieces) is cut into equal
+// parts for the warps of the block, whose sums are then added in order.
+constexpr int JOIN_WARPS = 8, LONG_RUN = 16;
+
 template <int V>
-__global__ void __launch_bounds__(SUM_WARPS * 32)
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
 join_runs_kernel(float* __restrict__ dtable, const float* __restrict__ carry, const int32_t* __restrict__ sorted_id,
                  int n, int vocab, int D, int pieces, float scale, int accumulate) {
     using TL = Tile<NVQ_F32, V>;
-    const int lane = threadIdx.x & 31;
-    const int piece = blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
-    if (piece + 1 >= pieces) return;
-    const int i0 = piece * PIECE, i1 = i0 + PIECE;      // i1 < n: another piece follows
-    const int id = sorted_id[i1 - 1];
-    if (id >= vocab || sorted_id[i1] != id) return;
-    if (sorted_id[i0] == id && i0 > 0 && sorted_id[i0 - 1] == id) return;     // began earlier
+    __shared__ int run_pieces[JOIN_WARPS];      // pieces after the first, for the block to add up; 0: none
+    __shared__ float part[JOIN_WARPS][TL::COLS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c0 = blockIdx.y * TL::COLS;
-    float acc[TL::E];
     auto fetch = [&](const float* row, float* f) {
 #pragma unroll
         for (int k = 0; k < TL::NV; k++) {
@@ -382,28 +385,68 @@ join_runs_kernel(float* __restrict__ dtable, const float* __restrict__ carry, co
             q.widen(f + k * V);
         }
     };
-    fetch(carry + ((size_t)piece * 2 + 1) * D, acc);
-    // pieces piece + 1 ... : a piece belongs to the run while its first token has the run's id
-    for (int q0 = piece + 1; q0 < pieces; q0 += 32) {
-        const int mine = q0 + lane;
-        const bool in = mine < pieces && sorted_id[(size_t)mine * PIECE] == id;
-        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, in);
-        const int many = hit == 0xFFFFFFFFu ? 32 : __ffs(~hit) - 1;
+    auto add_slots = [&](float* acc, int first, int many) {       // slot 0 of `many` pieces from `first`
         constexpr int AHEAD = 8;
         for (int a0 = 0; a0 < many; a0 += AHEAD) {
             float f[AHEAD][TL::E];
 #pragma unroll
             for (int a = 0; a < AHEAD; a++)
-                if (a0 + a < many) fetch(carry + (size_t)(q0 + a0 + a) * 2 * D, f[a]);
+                if (a0 + a < many) fetch(carry + (size_t)(first + a0 + a) * 2 * D, f[a]);
 #pragma unroll
             for (int a = 0; a < AHEAD; a++)
                 if (a0 + a < many)
 #pragma unroll
                     for (int e = 0; e < TL::E; e++) acc[e] += f[a][e];
         }
-        if (many < 32) break;
+    };
+    const int piece0 = blockIdx.x * JOIN_WARPS;
+    const int piece = piece0 + warp;
+    int many = 0, id = vocab;
+    if (piece + 1 < pieces) {
+        const int i0 = piece * PIECE, i1 = i0 + PIECE;      // i1 < n: another piece follows
+        id = sorted_id[i1 - 1];
+        const bool begins = id < vocab && sorted_id[i1] == id &&
+                            !(sorted_id[i0] == id && i0 > 0 && sorted_id[i0 - 1] == id);
+        // a piece belongs to the run while its first token has the run's id
+        for (int q0 = piece + 1; begins && q0 < pieces; q0 += 32) {
+            const int mine = q0 + lane;
+            const bool in = mine < pieces && sorted_id[(size_t)mine * PIECE] == id;
+            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, in);
+            many += hit == 0xFFFFFFFFu ? 32 : __ffs(~hit) - 1;
+            if (hit != 0xFFFFFFFFu) break;
+        }
     }
-    put_row<NVQ_F32, V>(dtable + (size_t)id * D, acc, c0, lane, D, scale, accumulate);
+    if (many > 0 && many <= LONG_RUN) {
+        float acc[TL::E];
+        fetch(carry + ((size_t)piece * 2 + 1) * D, acc);
+        add_slots(acc, piece + 1, many);
+        put_row<NVQ_F32, V>(dtable + (size_t)id * D, acc, c0, lane, D, scale, accumulate);
+    }
+    if (lane == 0) run_pieces[warp] = many > LONG_RUN ? many : 0;
+    __syncthreads();
+    for (int w = 0; w < JOIN_WARPS; w++) {
+        const int total = run_pieces[w];
+        if (total == 0) continue;
+        const int each = (total + JOIN_WARPS - 1) / JOIN_WARPS;
+        const int first = warp * each, mine = max(0, min(each, total - first));
+        float acc[TL::E];
+#pragma unroll
+        for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
+        if (warp == 0) fetch(carry + ((size_t)(piece0 + w) * 2 + 1) * D, acc);
+        add_slots(acc, piece0 + w + 1 + first, mine);
+#pragma unroll
+        for (int e = 0; e < TL::E; e++) part[warp][e * 32 + lane] = acc[e];
+        __syncthreads();
+        if (warp == w) {
+#pragma unroll
+            for (int e = 0; e < TL::E; e++) {
+                acc[e] = part[0][e * 32 + lane];
+                for (int x = 1; x < JOIN_WARPS; x++) acc[e] += part[x][e * 32 + lane];
+            }
+            put_row<NVQ_F32, V>(dtable + (size_t)id * D, acc, c0, lane, D, scale, accumulate);
+        }
+        __syncthreads();
+    }
 }
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
@@ -426,7 +469,10 @@ nvq_status sum_runs(float* dtable, float* carry, const char* dout, const int32_t
     const int pieces = (n + PIECE - 1) / PIECE;
     const bool wide = D % V16 == 0 && nvq_aligned(dout, 16) && nvq_aligned(dtable, 16);
     const dim3 block(SUM_WARPS * 32);
-    auto grid = [&](int cols) { return dim3((pieces + SUM_WARPS - 1) / SUM_WARPS, (D + cols - 1) / cols); };
+    auto grid = [&](int cols, int warps = SUM_WARPS) {
+        return dim3((pieces + warps - 1) / warps, (D + cols - 1) / cols);
+    };
+    const int join = JOIN_WARPS * 32;
     if (wide)
         sum_runs_kernel<DT, V16><<<grid(Tile<DT, V16>::COLS), block, 0, st>>>(dtable, carry, dout, sid, spos, n, vocab,
                                                                               D, pieces, scale, accumulate);
@@ -439,11 +485,11 @@ nvq_status sum_runs(float* dtable, float* carry, const char* dout, const int32_t
     NVQ_LAUNCHED();
     if (pieces > 1) {
         if (D % 4 == 0 && nvq_aligned(dtable, 16))
-            join_runs_kernel<4><<<grid(Tile<NVQ_F32, 4>::COLS), block, 0, st>>>(dtable, carry, sid, n, vocab, D, pieces,
-                                                                                scale, accumulate);
+            join_runs_kernel<4><<<grid(Tile<NVQ_F32, 4>::COLS, JOIN_WARPS), join, 0, st>>>(
+                dtable, carry, sid, n, vocab, D, pieces, scale, accumulate);
         else
-            join_runs_kernel<1><<<grid(Tile<NVQ_F32, 1>::COLS), block, 0, st>>>(dtable, carry, sid, n, vocab, D, pieces,
-                                                                                scale, accumulate);
+            join_runs_kernel<1><<<grid(Tile<NVQ_F32, 1>::COLS, JOIN_WARPS), join, 0, st>>>(
+                dtable, carry, sid, n, vocab, D, pieces, scale, accumulate);
         NVQ_LAUNCHED();
     }
     return NVQ_OK;

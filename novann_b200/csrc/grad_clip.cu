@@ -143,7 +143,7 @@ __device__ __forceinline__ void chunk_scale(void* d, const void* p, int n, bool 
         Packet<DT, V> q[ROUNDS];
 #pragma unroll
         for (int i = 0; i < ROUNDS; i++)
-            q[i].load((const char*)p + (size_t)(i * THREADS + threadIdx.x) * 16);
+            q[i].load_once((const char*)p + (size_t)(i * THREADS + threadIdx.x) * 16);
 #pragma unroll
         for (int i = 0; i < ROUNDS; i++) {
             float f[V];

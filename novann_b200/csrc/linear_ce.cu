@@ -1,0 +1,892 @@
+// Softmax cross entropy of a linear layer's output, the logits never kept.
+//
+//   l = X W^T + b;   lse_m = log sum_v exp(l_mv);   loss_m = lse_m - l_m,y(m)   (rows that count)
+//   g = s (exp(l - lse) - onehot(y)),  s = grad_scale / (rows that count, or 1 for a sum)
+//   dX = g W,  dW = g^T X,  db = sum over m of g
+//
+// One kernel does all four contractions: a pair of CTAs per 256 x 256 output tile, operands by TMA into
+// a six-stage ring, tcgen05.mma (cta_group::2) into two TMEM accumulators, so that the epilogue of one
+// tile runs under the MMAs of the next.  What differs is which of an operand's two dimensions is
+// contiguous (the contraction for X W^T and for g in dX; the other one for W in dX and for both
+// operands of dW - the tensor core reads either, so nothing is ever transposed) and the epilogue:
+//   kLse   per row the maximum and the sum of exp over 128 columns, and the label's logit
+//   kProb  softmax(l) - onehot as 16-bit values, a piece of the vocabulary at a time
+//   kSum   fp32 sums: added to a buffer, or scaled and rounded to the gradient's type
+// The backward pass computes the logits of a piece a second time instead of keeping M x V of them:
+// 8 M V K operations where 6 M V K are needed, against reading and writing the logits twice.
+#include "gemm_common.cuh"
+#include "packet.cuh"
+
+namespace {
+
+constexpr int BM = 256, BN = 256, BK = 64, UMMA_K = 16;
+constexpr int A_BYTES = 128 * BK * 2, B_BYTES = 128 * BK * 2;   // per CTA
+constexpr int STAGES = 6;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 8192;
+constexpr int TMEM_COLS = 512;
+constexpr float LOG2E = 1.4426950408889634f;
+// fp16 values of g below 2^-14 would lose bits: they are kept times 2^14 (|g| <= 1 stays in range)
+constexpr float F16_GAIN = 16384.f;
+
+enum { kLse = 0, kProb = 1, kSum = 2 };
+enum { ERR_PRODUCER = 81, ERR_MMA_FULL = 82, ERR_MMA_TMEM = 83, ERR_EPILOGUE = 84, ERR_LABEL = 85 };
+
+struct CeParams : LinearParams {
+    int splits, kb_per;          // the contraction cut into `splits` parts of kb_per k-blocks
+    int f16;                     // operands are fp16 (else bf16)
+    // kLse, kProb
+    const int32_t* labels;
+    float2* partial;             // kLse: (2 * n_blocks) x M maxima and sums
+    float* label_logit;          // kLse: M
+    const float* stats;          // kProb: M row maxima, then M logarithms of the sums of exp(l - maximum)
+    int v0, vocab, ignore;       // kProb: first vocabulary entry of this piece, vocabulary, label that does not count
+    uint16_t* prob;              // kProb: M x ldp, ldp a multiple of 16, 0 past the piece
+    int ldp;
+    float* col_partial;          // kProb: ceil(M / 32) x ldp column sums of 32 rows each, or nullptr
+    // kSum
+    const float* add;            // fp32 sums of earlier pieces (M x N), or nullptr
+    float* sum;                  // where fp32 sums go (M x N each; split s at s * M * N), or nullptr
+    void* out;                   // final result in out_type, or nullptr
+    int out_type;
+    int vec32;                   // out's rows start on 32-byte boundaries
+    float scale;                 // factor of the final result, over the count of rows where `count` is set
+    const float* count;
+};
+
+struct Shared {
+    uint64_t full[STAGES];
+    uint64_t empty[STAGES];
+    uint64_t tmem_full[4];
+    uint64_t tmem_empty[4];
+    uint32_t tmem_base;
+    int abort_flag;
+    alignas(16) float bias[2][BN];
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Shared-memory descriptor of a tile whose rows run along the contraction and hold 64 elements of the
+// other dimension (128 bytes, 128-byte swizzle): groups of 8 rows are 1024 bytes apart, the next 64
+// elements of the other dimension 64 rows (8192 bytes) further on.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(8192 >> 4) << 16;                      // leading byte offset
+    d |= (uint64_t)(1024 >> 4) << 32;                      // stride byte offset
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+struct Item { TileRef tile; int kb0, kb1, split; };
+__device__ __forceinline__ Item item_of(const CeParams& p, int t, int num_kb) {
+    Item it;
+    it.split = 0;
+    it.kb0 = 0;
+    it.kb1 = num_kb;
+    if (p.splits > 1) {          // num_items = tiles * splits, a tile's parts next to one another
+        it.split = t % p.splits;
+        t /= p.splits;
+        it.kb0 = it.split * p.kb_per;
+        it.kb1 = min(num_kb, it.kb0 + p.kb_per);
+    }
+    it.tile = tile_ref(p, t);
+    return it;
+}
+
+// 32 fp32 sums of one row (columns n ...): to the fp32 buffer, or scaled to the final type
+__device__ __forceinline__ void store_sum(const CeParams& p, const uint32_t* r, size_t at, int n, int split, float s) {
+    if (p.out == nullptr || p.out_type == NVQ_F32) {
+        float* dst = p.out ? (float*)p.out + at : p.sum + (size_t)split * p.M * p.N + at;
+        const bool wide = p.out == nullptr || p.vec32;
+#pragma unroll
+        for (int g = 0; g < 32; g += 8) {
+            if (n + g >= p.N) break;
+            u32x8 o;
+#pragma unroll
+            for (int j = 0; j < 8; j++) o.v[j] = __float_as_uint(__uint_as_float(r[g + j]) * s);
+            if (wide) {
+                stg_stream_256(dst + g, o);
+            } else {
+                stg_stream_128(dst + g, make_uint4(o.v[0], o.v[1], o.v[2], o.v[3]));
+                stg_stream_128(dst + g + 4, make_uint4(o.v[4], o.v[5], o.v[6], o.v[7]));
+            }
+        }
+    } else {
+        uint16_t* dst = (uint16_t*)p.out + at;
+#pragma unroll
+        for (int g = 0; g < 32; g += 16) {
+            if (n + g >= p.N) break;
+            u32x8 o;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float a = __uint_as_float(r[g + 2 * j]) * s, b = __uint_as_float(r[g + 2 * j + 1]) * s;
+                o.v[j] = p.out_type == NVQ_F16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+            }
+            if (p.vec32 && n + g + 16 <= p.N) {
+                stg_stream_256(dst + g, o);
+            } else {
+                stg_stream_128(dst + g, make_uint4(o.v[0], o.v[1], o.v[2], o.v[3]));
+                if (n + g + 16 <= p.N) stg_stream_128(dst + g + 8, make_uint4(o.v[4], o.v[5], o.v[6], o.v[7]));
+            }
+        }
+    }
+}
+
+// A_MN / B_MN: the operand is stored with its own dimension contiguous instead of the contraction's
+template <int EPI, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const CeParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = tc::smem_u32(smem_raw);
+    const uint32_t tiles = (raw + 1023u) & ~1023u;
+    Shared* sh = (Shared*)(smem_raw + (tiles - raw) + STAGES * STAGE_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_ctarank();
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const int num_kb = (p.K + BK - 1) / BK;
+    volatile int* abort_flag = &sh->abort_flag;
+    // accumulators: two of 256 columns, or four of 128 when the output has at most 128 columns
+    const bool narrow = p.N <= BN / 2;
+    const uint32_t acc_cols = narrow ? BN / 2 : BN;
+    auto acc_of = [&](int it, uint32_t& acc, uint32_t& acc_phase) {
+        if (narrow) { acc = it & 3; acc_phase = (it >> 2) & 1; }
+        else        { acc = it & 1; acc_phase = (it >> 1) & 1; }
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            tc::mbar_init(tc::smem_u32(&sh->full[s]), 1);
+            tc::mbar_init(tc::smem_u32(&sh->empty[s]), 1);
+        }
+        for (int a = 0; a < 4; a++) {
+            tc::mbar_init(tc::smem_u32(&sh->tmem_full[a]), 1);
+            tc::mbar_init(tc::smem_u32(&sh->tmem_empty[a]), 2 * EPI_WARPS);
+        }
+        sh->abort_flag = 0;
+        tc::mbar_fence_init();
+        tc::tma_prefetch_desc(&map_a);
+        tc::tma_prefetch_desc(&map_b);
+    }
+    if (warp == 1) {
+        tc::tmem_alloc_pair(tc::smem_u32(&sh->tmem_base), TMEM_COLS);
+        tc::tmem_relinquish_pair();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::cluster_sync_all();
+    tc::tc_fence_after();
+    const uint32_t tmem_base = sh->tmem_base;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer (both CTAs)
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (int t = pair; t < p.num_items && ok; t += num_pairs) {
+                const Item it = item_of(p, t, num_kb);
+                const int rows_b = it.tile.is_half ? BN / 4 : BN / 2;       // per CTA
+                const int m0 = it.tile.m_blk * BM + (int)rank * 128;
+                const int n0 = it.tile.n_blk * BN + it.tile.half * (BN / 2) + (int)rank * rows_b;
+                for (int kb = it.kb0; kb < it.kb1; kb++) {
+                    ok = tc::mbar_wait(tc::smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, ERR_PRODUCER);
+                    if (!ok) break;
+                    const uint32_t dst = tiles + stage * STAGE_BYTES;
+                    const uint32_t lead_full = tc::mapa(tc::smem_u32(&sh->full[stage]), 0);
+                    if (rank == 0)       // the leader expects the bytes of both CTAs
+                        tc::mbar_arrive_expect_tx(tc::smem_u32(&sh->full[stage]), 2 * (A_BYTES + rows_b * BK * 2));
+                    if constexpr (A_MN) {
+                        tc::tma_load_2d_pair(dst, &map_a, lead_full, m0, kb * BK);
+                        tc::tma_load_2d_pair(dst + A_BYTES / 2, &map_a, lead_full, m0 + 64, kb * BK);
+                    } else {
+                        tc::tma_load_2d_pair(dst, &map_a, lead_full, kb * BK, m0);
+                    }
+                    if constexpr (B_MN) {
+                        tc::tma_load_2d_pair(dst + A_BYTES, &map_b, lead_full, n0, kb * BK);
+                        if (rows_b == 128)
+                            tc::tma_load_2d_pair(dst + A_BYTES + B_BYTES / 2, &map_b, lead_full, n0 + 64, kb * BK);
+                    } else {
+                        tc::tma_load_2d_pair(dst + A_BYTES, &map_b, lead_full, kb * BK, n0);
+                        if (rows_b == 128)
+                            tc::tma_load_2d_pair(dst + A_BYTES + B_BYTES / 2, &map_b, lead_full, kb * BK, n0 + 64);
+                    }
+                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer (leader only)
+        if (lane == 0 && rank == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true, ready = false;
+            int n = 0;
+            const uint32_t fmt = p.f16 ? 0u : 1u;
+            const uint32_t major = (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+            for (int t = pair; t < p.num_items && ok; t += num_pairs, n++) {
+                uint32_t acc, acc_phase;
+                acc_of(n, acc, acc_phase);
+                const Item it = item_of(p, t, num_kb);
+                const uint32_t idesc = tc::idesc_f16(BM, it.tile.is_half ? BN / 2 : BN, fmt, fmt) | major;
+                ok = tc::mbar_wait(tc::smem_u32(&sh->tmem_empty[acc]), acc_phase ^ 1, abort_flag, ERR_MMA_TMEM);
+                if (!ok) break;
+                tc::tc_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * acc_cols;
+                for (int kb = it.kb0; kb < it.kb1; kb++) {
+                    if (!ready) {
+                        ok = tc::mbar_wait(tc::smem_u32(&sh->full[stage]), phase, abort_flag, ERR_MMA_FULL);
+                        if (!ok) break;
+                    }
+                    tc::tc_fence_after();
+                    const uint32_t nstage = stage + 1 == (uint32_t)STAGES ? 0u : stage + 1;
+                    const uint32_t nphase = nstage == 0 ? phase ^ 1u : phase;
+                    const uint32_t a_addr = tiles + stage * STAGE_BYTES, b_addr = a_addr + A_BYTES;
+                    const uint64_t a_desc = A_MN ? smem_desc_mn_sw128(a_addr) : tc::smem_desc_k_sw128(a_addr);
+                    const uint64_t b_desc = B_MN ? smem_desc_mn_sw128(b_addr) : tc::smem_desc_k_sw128(b_addr);
+                    // 16 contraction steps: 32 bytes along a row, or 16 rows of 128 bytes
+                    constexpr uint32_t a_step = A_MN ? 2048 >> 4 : 32 >> 4, b_step = B_MN ? 2048 >> 4 : 32 >> 4;
+#pragma unroll
+                    for (int k = 0; k < BK / UMMA_K; k++) {
+                        tc::tc_mma_f16_pair(d_tmem, a_desc + a_step * k, b_desc + b_step * k, idesc,
+                                            kb > it.kb0 || k > 0);
+                        if (k == 0) ready = tc::mbar_test_wait(tc::smem_u32(&sh->full[nstage]), nphase);
+                    }
+                    tc::tc_commit_pair(tc::smem_u32(&sh->empty[stage]), 3);
+                    stage = nstage;
+                    phase = nphase;
+                }
+                if (ok) tc::tc_commit_pair(tc::smem_u32(&sh->tmem_full[acc]), 3);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue (both CTAs)
+        const int quarter = warp & 3;                 // the TMEM lanes this warp may read
+        const int colgrp = (warp - 2) >> 2;           // which 128 (64) columns of the tile
+        const int et = threadIdx.x - 64;              // 0 .. 255
+        bool ok = true;
+        int n_it = 0;
+        for (int t = pair; t < p.num_items && ok; t += num_pairs, n_it++) {
+            uint32_t acc, acc_phase;
+            acc_of(n_it, acc, acc_phase);
+            const Item it = item_of(p, t, num_kb);
+            const int bn = it.tile.is_half ? BN / 2 : BN;
+            const int m0 = it.tile.m_blk * BM + (int)rank * 128;
+            const int n0 = it.tile.n_blk * BN + it.tile.half * (BN / 2);
+            const int row = m0 + quarter * 32 + lane;
+            const bool valid = row < p.M;
+            float* bi = &sh->bias[0][0] + acc * acc_cols;
+            int label = -1;              // column of this launch, or out of its range
+            [[maybe_unused]] float row_max = 0.f, log2_sum = 0.f;
+            [[maybe_unused]] bool counts = false;
+            if constexpr (EPI != kSum) {
+                for (int c = et; c < bn; c += 32 * EPI_WARPS)
+                    bi[c] = p.bias && n0 + c < p.N ? p.bias[n0 + c] : 0.f;
+                if (valid) {
+                    if constexpr (EPI == kLse) {
+                        label = p.labels[row];
+                    } else {
+                        const int y = p.labels[row];
+                        row_max = p.stats[row];
+                        log2_sum = p.stats[(size_t)p.M + row] * LOG2E;
+                        // a row whose every entry is taken out (-inf) has no gradient
+                        counts = y != p.ignore && y >= 0 && y < p.vocab && row_max != -INFINITY;
+                        label = y - p.v0;
+                    }
+                }
+            }
+            [[maybe_unused]] float out_scale = 1.f;
+            if constexpr (EPI == kSum)
+                if (p.out) out_scale = p.count ? p.scale / fmaxf(*p.count, 1.f) : p.scale;
+            ok = tc::mbar_wait(tc::smem_u32(&sh->tmem_full[acc]), acc_phase, abort_flag, ERR_EPILOGUE);
+            ok = epilogue_all<32 * EPI_WARPS>(ok);
+            if (!ok) break;
+            tc::tc_fence_after();
+            const uint32_t taddr = tmem_base + acc * acc_cols + ((uint32_t)(quarter * 32) << 16);
+            const int c_first = colgrp * (bn / 2), c_end = c_first + bn / 2;
+            [[maybe_unused]] float top = -INFINITY, sum = 0.f;
+
+            auto emit = [&](uint32_t* r, int c) {      // 32 columns from tile column c
+                const int n = n0 + c;                  // output column
+                if constexpr (EPI == kSum) {
+                    if (!valid || n >= p.N) return;
+                    const size_t at = (size_t)row * p.N + n;
+#pragma unroll
+                    for (int g = 0; g < 32; g += 8) {
+                        if (n + g >= p.N) break;       // N % 8 == 0: groups of eight are in or out together
+                        if (p.add) {
+                            float a[8];
+                            load8_f32(a, p.add + at + g);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) r[g + j] = __float_as_uint(__uint_as_float(r[g + j]) + a[j]);
+                        }
+                    }
+                    store_sum(p, r, at, n, it.split, out_scale);
+                } else {
+                    float f[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        float b8[8];
+                        load8_f32(b8, bi + c + j);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) f[j + i] = __uint_as_float(r[j + i]) + b8[i];
+                    }
+                    if (n + 32 > p.N) {                 // past the vocabulary: exp(-inf) = 0
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (n + j >= p.N) f[j] = -INFINITY;
+                    }
+                    const int hit = label - n;          // the label's place in this chunk
+                    if constexpr (EPI == kLse) {
+                        if (hit >= 0 && hit < 32 && label < p.N) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (j == hit) p.label_logit[row] = f[j];
+                        }
+                        float m = f[0];
+#pragma unroll
+                        for (int j = 1; j < 32; j++) m = fmaxf(m, f[j]);
+                        m = fmaxf(m, top);
+                        // a row whose entries are all masked so far (-inf) has sum 0 relative to 0
+                        const float ref = m == -INFINITY ? 0.f : m;
+                        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            s0 += ex2((f[j] - ref) * LOG2E);
+                            s1 += ex2((f[j + 1] - ref) * LOG2E);
+                            s2 += ex2((f[j + 2] - ref) * LOG2E);
+                            s3 += ex2((f[j + 3] - ref) * LOG2E);
+                        }
+                        sum = sum * ex2((top - ref) * LOG2E) + ((s0 + s1) + (s2 + s3));
+                        top = m;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) f[j] = ex2(fmaf(f[j] - row_max, LOG2E, -log2_sum));
+                        if (hit >= 0 && hit < 32) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (j == hit) f[j] -= 1.f;
+                        }
+                        // a row that does not count gives zeros whatever its logits are
+#pragma unroll
+                        for (int j = 0; j < 32; j++) f[j] = counts ? f[j] : 0.f;
+                        if (valid && n < p.ldp) {
+                            uint16_t* dst = p.prob + (size_t)row * p.ldp + n;
+#pragma unroll
+                            for (int g = 0; g < 32; g += 16) {
+                                if (n + g >= p.ldp) break;
+                                u32x8 o;
+#pragma unroll
+                                for (int j = 0; j < 8; j++) {
+                                    const float a = f[g + 2 * j], b = f[g + 2 * j + 1];
+                                    o.v[j] = p.f16 ? pack_f16x2(a * F16_GAIN, b * F16_GAIN) : pack_bf16x2(a, b);
+                                }
+                                stg_stream_256(dst + g, o);
+                            }
+                        }
+                        if (p.col_partial) {
+                            // Sums of 32 columns over the warp's 32 rows: at each step a lane keeps the half of
+                            // its columns that its lane bit names and adds its partner's; after five steps
+                            // lane l holds column l.
+#pragma unroll
+                            for (int h = 16; h; h >>= 1) {
+                                const bool upper = (lane & h) != 0;
+#pragma unroll
+                                for (int j = 0; j < h; j++) {
+                                    const float keep = upper ? f[j + h] : f[j], give = upper ? f[j] : f[j + h];
+                                    f[j] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, h);
+                                }
+                            }
+                            if (n + lane < p.ldp && m0 + quarter * 32 < p.M)
+                                p.col_partial[(size_t)((m0 >> 5) + quarter) * p.ldp + n + lane] = f[0];
+                        }
+                    }
+                }
+            };
+            // a chunk is loaded from TMEM while the one before it is worked on
+            uint32_t ra[32], rb[32];
+            tc::tmem_ld_32x32(taddr + c_first, ra);
+#pragma unroll 1
+            for (int c = c_first; c < c_end; c += 64) {
+                tc::tmem_ld_wait();
+                if (c + 32 < c_end) tc::tmem_ld_32x32(taddr + c + 32, rb);
+                emit(ra, c);
+                if (c + 32 < c_end) {
+                    tc::tmem_ld_wait();
+                    if (c + 64 < c_end) tc::tmem_ld_32x32(taddr + c + 64, ra);
+                    emit(rb, c + 32);
+                }
+            }
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive_remote(tc::mapa(tc::smem_u32(&sh->tmem_empty[acc]), 0));
+            // the joined maximum and sum of this warp's columns, for each of its rows (kLse tiles are never
+            // cut in two, so a 256-column block has these two entries)
+            if constexpr (EPI == kLse)
+                if (valid) p.partial[(size_t)(it.tile.n_blk * 2 + colgrp) * p.M + row] = make_float2(top, sum);
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    if (*abort_flag) {
+        for (int i = 0; i < 64; i++) __nanosleep(20000);
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::cluster_sync_all();
+    tc::tc_fence_after();
+    if (warp == 1) tc::tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    if (threadIdx.x == 0 && *abort_flag && p.status) atomicCAS(p.status, 0, *abort_flag);
+}
+
+// ---------------------------------------------------------------- joining what the tiles left
+// Row statistics, row loss and the label checks: 32 rows per block, one per lane, the partial maxima and sums
+// dealt out to the warps.  The sum of the block's row losses and its count of rows go to block_sum.
+constexpr int JOIN_WARPS = 32;
+
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+    const float top = fmaxf(m, m2);
+    const float ref = top == -INFINITY ? 0.f : top;
+    s = s * ex2((m - ref) * LOG2E) + s2 * ex2((m2 - ref) * LOG2E);
+    m = top;
+}
+
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+join_lse_kernel(float* __restrict__ stats, float* __restrict__ row_loss, float2* __restrict__ block_sum,
+                const float2* __restrict__ partial, const float* __restrict__ label_logit,
+                const int32_t* __restrict__ labels, int M, int slots, int vocab, int ignore, int* __restrict__ status) {
+    __shared__ float2 part[JOIN_WARPS][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = blockIdx.x * 32 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float m = -INFINITY, s = 0.f;
+    if (row < M) {
+        int i = warp;
+        for (; i + 3 * JOIN_WARPS < slots; i += 4 * JOIN_WARPS) {
+            float2 q[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) q[k] = partial[(size_t)(i + k * JOIN_WARPS) * M + row];
+#pragma unroll
+            for (int k = 0; k < 4; k++) join(m, s, q[k].x, q[k].y);
+        }
+        for (; i < slots; i += JOIN_WARPS) {
+            const float2 q = partial[(size_t)i * M + row];
+            join(m, s, q.x, q.y);
+        }
+    }
+    part[warp][lane] = make_float2(m, s);
+    __syncthreads();
+    if (warp != 0) return;
+    for (int w = 1; w < JOIN_WARPS; w++) join(m, s, part[w][lane].x, part[w][lane].y);
+    float loss = 0.f, n = 0.f;
+    if (row < M) {
+        // maximum and logarithm are kept apart: their sum would lose the logarithm where the logits are large
+        const float log_sum = m == -INFINITY ? 0.f : logf(s);
+        const int y = labels[row];
+        if (y != ignore) {
+            if (y >= 0 && y < vocab) {
+                loss = m == -INFINITY ? INFINITY : (m - label_logit[row]) + log_sum;
+                n = 1.f;
+            } else if (status) {
+                atomicCAS(status, 0, (int)ERR_LABEL);
+            }
+        }
+        stats[row] = m;
+        stats[(size_t)M + row] = log_sum;
+        if (row_loss) row_loss[row] = loss;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        loss += __shfl_xor_sync(0xFFFFFFFFu, loss, o);
+        n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
+    }
+    if (lane == 0) block_sum[blockIdx.x] = make_float2(loss, n);
+}
+
+// loss[0] = sum of the row losses (over their count for the mean; 0 when no row counts), loss[1] = count
+__global__ void __launch_bounds__(256)
+loss_kernel(float* __restrict__ loss, const float2* __restrict__ block_sum, int blocks, int mean) {
+    __shared__ double sum[8], num[8];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    double s = 0.0, n = 0.0;
+    for (int i = threadIdx.x; i < blocks; i += 256) {
+        s += block_sum[i].x;
+        n += block_sum[i].y;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+        n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
+    }
+    if ((threadIdx.x & 31) == 0) { sum[threadIdx.x >> 5] = s; num[threadIdx.x >> 5] = n; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; w++) { s += sum[w]; n += num[w]; }
+        loss[0] = (float)(mean ? s / (n > 1.0 ? n : 1.0) : s);
+        loss[1] = (float)n;
+    }
+}
+
+// (sum of the parts of a split contraction + add) -> fp32 buffer, or scaled to the final type; n % 8 == 0
+template <int DT>
+__global__ void __launch_bounds__(256)
+join_splits_kernel(void* out, const float* __restrict__ parts, int splits, const float* add, size_t n,
+                   float scale, const float* __restrict__ count) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; s++) {
+        const float4 v = *(const float4*)(parts + (size_t)s * n + i);
+        f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
+    }
+    if (add) {
+        const float4 v = *(const float4*)(add + i);
+        f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
+    }
+    const float s = count ? scale / fmaxf(*count, 1.f) : scale;
+#pragma unroll
+    for (int j = 0; j < 4; j++) f[j] *= s;
+    if constexpr (DT == NVQ_F32) {
+        *(float4*)((float*)out + i) = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+        *(uint2*)((uint16_t*)out + i) = make_uint2(Elem<DT>::narrow(f), Elem<DT>::narrow(f + 2));
+    }
+}
+
+// db = scale * the column sums' sum over the groups of 32 rows
+__global__ void __launch_bounds__(256)
+bias_grad_kernel(float* __restrict__ db, const float* __restrict__ col_partial, int groups, int ld, int N, float scale,
+                 const float* __restrict__ count) {
+    __shared__ float part[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c = blockIdx.x * 32 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float s = 0.f;
+    if (c < N)
+#pragma unroll 4
+        for (int g = warp; g < groups; g += 8) s += col_partial[(size_t)g * ld + c];
+    part[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < N) {
+        for (int w = 1; w < 8; w++) s += part[w][lane];
+        db[c] = s * (count ? scale / fmaxf(*count, 1.f) : scale);
+    }
+}
+
+// ---------------------------------------------------------------- host
+template <typename... KArgs, typename... Args>
+nvq_status launch_after(void (*kernel)(KArgs...), size_t grid, int threads, int smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // may start under the tail
+    attr[0].val.programmaticStreamSerializationAllowed = 1;            // of the previous kernel
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    NVQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...));
+    NVQ_LAUNCHED();
+    return NVQ_OK;
+}
+
+template <int EPI, bool A_MN, bool B_MN>
+nvq_status launch_gemm(CeParams& p, const CUtensorMap& a, const CUtensorMap& b, int device, cudaStream_t st) {
+    static std::atomic<bool> attr_set[64];   // per device; setting the attribute twice is harmless
+    if (!attr_set[device]) {
+        NVQ_CUDA(cudaFuncSetAttribute(ce_gemm_kernel<EPI, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      SMEM_BYTES));
+        attr_set[device] = true;
+    }
+    nvq_status s = nvq_status_word(device, &p.status);
+    if (s != NVQ_OK) return s;
+    p.m_blocks = (p.M + BM - 1) / BM;
+    p.n_blocks = (p.N + BN - 1) / BN;
+    p.group_m = 8;
+    const int tiles = p.m_blocks * p.n_blocks, pairs = nvq_sm_count(device) / 2;
+    p.num_big = p.num_items = tiles * p.splits;
+    if (EPI != kLse && p.splits == 1 && p.N > BN / 2) {
+        // a partial last wave that would occupy at most half of the pairs is cut into half-width tiles
+        const int rem = tiles % pairs;
+        const int cut = tiles > pairs && rem > 0 && 2 * rem <= pairs ? rem : 0;
+        p.num_big = tiles - cut;
+        p.num_items = p.num_big + 2 * cut;
+    }
+    const int used = p.num_items < pairs ? p.num_items : pairs;
+    return launch_after(ce_gemm_kernel<EPI, A_MN, B_MN>, 2 * (size_t)used, THREADS, SMEM_BYTES, st, a, b, p);
+}
+
+size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+
+// A contraction with fewer output tiles than half the CTA pairs is cut along its length, four k-blocks
+// at least in a part, so that every pair has one.
+struct Split { int splits, kb_per; };
+Split split_of(size_t M, size_t N, size_t K, int pairs) {
+    const size_t tiles = (M + BM - 1) / BM * ((N + BN - 1) / BN);
+    const int num_kb = (int)((K + BK - 1) / BK);
+    int want = tiles * 2 > (size_t)pairs ? 1 : (int)(pairs / tiles);
+    if (want > num_kb / 4) want = num_kb / 4;
+    if (want < 1) want = 1;
+    Split s;
+    s.kb_per = (num_kb + want - 1) / want;
+    s.splits = (num_kb + s.kb_per - 1) / s.kb_per;
+    return s;
+}
+
+// Vocabulary entries per piece of the backward pass: 64 Mi values of g, 8192 entries at least, so that adding a
+// piece to the fp32 dX costs little beside its contractions.
+size_t piece_of(size_t M, size_t V) {
+    size_t most = ((size_t)64 << 20) / M;
+    if (most < 8192) most = 8192;
+    const size_t pieces = (V + most - 1) / most;
+    const size_t each = (V + pieces - 1) / pieces;
+    return (each + 255) / 256 * 256;
+}
+
+struct FwdSpace { size_t partial, logit, block, total; };
+FwdSpace fwd_space(size_t M, size_t V) {
+    FwdSpace s;
+    s.partial = align256((V + BN - 1) / BN * 2 * M * sizeof(float2));
+    s.logit = align256(M * 4);
+    s.block = align256((M + 31) / 32 * sizeof(float2));
+    s.total = s.partial + s.logit + s.block;
+    return s;
+}
+struct BwdSpace { size_t prob, cols, sum, parts, total; };
+BwdSpace bwd_space(size_t M, size_t V, size_t K, int pairs) {
+    BwdSpace s;
+    const size_t piece = piece_of(M, V), nv = piece < V ? piece : V, ld = (nv + 15) / 16 * 16;
+    s.prob = align256(M * ld * 2);
+    s.cols = align256((M + 31) / 32 * ld * 4);
+    s.sum = piece < V ? align256(M * K * 4) : 0;
+    const Split x = split_of(M, K, nv, pairs), w = split_of(nv, K, M, pairs);
+    const size_t px = x.splits > 1 ? x.splits * M * K * 4 : 0, pw = w.splits > 1 ? w.splits * nv * K * 4 : 0;
+    // the last piece may be shorter, and its split another one: its parts are never more than a wave of tiles
+    const size_t wave = (size_t)pairs * BM * BN * 4;
+    size_t parts = px > pw ? px : pw;
+    if (piece < V && parts < wave) parts = wave;
+    s.parts = align256(parts);
+    s.total = s.prob + s.cols + s.sum + s.parts;
+    return s;
+}
+
+constexpr int kDefaultPairs = 74;      // sizes are asked for without a device
+
+template <bool A_MN, bool B_MN>
+nvq_status contract(CeParams& p, const CUtensorMap& a, const CUtensorMap& b, float* parts, int device, cudaStream_t st) {
+    const Split sp = split_of(p.M, p.N, p.K, kDefaultPairs);
+    p.splits = sp.splits;
+    p.kb_per = sp.kb_per;
+    if (sp.splits == 1) return launch_gemm<kSum, A_MN, B_MN>(p, a, b, device, st);
+    CeParams q = p;
+    q.out = nullptr;
+    q.add = nullptr;
+    q.sum = parts;
+    nvq_status s = launch_gemm<kSum, A_MN, B_MN>(q, a, b, device, st);
+    if (s != NVQ_OK) return s;
+    const size_t n = (size_t)p.M * p.N, grid = (n / 4 + 255) / 256;
+    if (p.out == nullptr)
+        return launch_after(join_splits_kernel<NVQ_F32>, grid, 256, 0, st, (void*)p.sum, parts, sp.splits, p.add, n, 1.f,
+                            nullptr);
+    if (p.out_type == NVQ_F32)
+        return launch_after(join_splits_kernel<NVQ_F32>, grid, 256, 0, st, p.out, parts, sp.splits, p.add, n, p.scale,
+                            p.count);
+    if (p.out_type == NVQ_F16)
+        return launch_after(join_splits_kernel<NVQ_F16>, grid, 256, 0, st, p.out, parts, sp.splits, p.add, n, p.scale,
+                            p.count);
+    return launch_after(join_splits_kernel<NVQ_BF16>, grid, 256, 0, st, p.out, parts, sp.splits, p.add, n, p.scale,
+                        p.count);
+}
+
+nvq_status check_shape(const char* who, const void* x, const void* w, int dtype, const float* bias,
+                       const int32_t* labels, size_t M, size_t V, size_t K, int reduction) {
+    NVQ_REQUIRE(dtype == NVQ_BF16 || dtype == NVQ_F16, "%s: operand type %d; f16 and bf16 are taken", who, dtype);
+    NVQ_REQUIRE(V > 0 && K > 0 && M <= (1u << 30) && V <= (1u << 30) && K <= (1u << 20),
+                "%s: M up to 2^30, V in [1, 2^30], K in [1, 2^20]", who);
+    NVQ_REQUIRE(K % 8 == 0, "%s: K (%zu) must be a multiple of 8", who, K);
+    NVQ_REQUIRE((M + BM - 1) / BM * ((V + BN - 1) / BN) < ((size_t)1 << 30), "%s: M * V is too large", who);
+    NVQ_REQUIRE(reduction == NVQ_REDUCE_SUM || reduction == NVQ_REDUCE_MEAN, "%s: unknown reduction %d", who, reduction);
+    NVQ_REQUIRE(w && nvq_aligned(w, 16) && (M == 0 || (x && nvq_aligned(x, 16))), "%s: x and w must be 16-byte aligned",
+                who);
+    NVQ_REQUIRE(M == 0 || (labels && nvq_aligned(labels, 4)), "%s: null or misaligned labels", who);
+    NVQ_REQUIRE(nvq_aligned(bias, 4), "%s: misaligned bias", who);
+    return NVQ_OK;
+}
+
+}  // namespace
+
+extern "C" nvq_status nvq_linear_ce_workspace_bytes(size_t M, size_t V, size_t K, int backward, size_t* bytes) {
+    NVQ_REQUIRE(bytes, "null out pointer");
+    NVQ_REQUIRE(V > 0 && K > 0 && M <= (1u << 30) && V <= (1u << 30) && K <= (1u << 20),
+                "nvq_linear_ce_workspace_bytes: M up to 2^30, V in [1, 2^30], K in [1, 2^20]");
+    *bytes = 0;
+    if (M == 0) return NVQ_OK;
+    *bytes = fwd_space(M, V).total;
+    if (backward) {
+        const size_t b = bwd_space(M, V, K, kDefaultPairs).total;
+        if (b > *bytes) *bytes = b;
+    }
+    return NVQ_OK;
+}
+
+extern "C" nvq_status nvq_linear_ce_fwd(float* d_loss_count, float* d_row_loss, float* d_row_stats, const void* d_x,
+                                        const void* d_w, nvq_dtype dtype, const float* d_bias, const int32_t* d_labels,
+                                        size_t M, size_t V, size_t K, int32_t ignore_index, int reduction,
+                                        void* d_workspace, size_t workspace_bytes, int device, void* stream) {
+    nvq_status s = check_shape("nvq_linear_ce_fwd", d_x, d_w, dtype, d_bias, d_labels, M, V, K, reduction);
+    if (s != NVQ_OK) return s;
+    NVQ_REQUIRE(d_loss_count && nvq_aligned(d_loss_count, 4) && nvq_aligned(d_row_loss, 4) &&
+                    (M == 0 || (d_row_stats && nvq_aligned(d_row_stats, 4))),
+                "nvq_linear_ce_fwd: null or misaligned output");
+    const FwdSpace sp = fwd_space(M, V);
+    NVQ_REQUIRE(M == 0 || (d_workspace && workspace_bytes >= sp.total && nvq_aligned(d_workspace, 256)),
+                "nvq_linear_ce_fwd: workspace of %zu bytes (256-byte aligned) required", sp.total);
+    s = nvq_use_device(device);
+    if (s != NVQ_OK) return s;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (M == 0) {
+        NVQ_CUDA(cudaMemsetAsync(d_loss_count, 0, 2 * sizeof(float), st));
+        return NVQ_OK;
+    }
+    CUtensorMap a, b;
+    s = nvq_make_tmap_2d(&a, d_x, M, K, 128, BK, 2, 1);
+    if (s != NVQ_OK) return s;
+    s = nvq_make_tmap_2d(&b, d_w, V, K, 64, BK, 2, 1);
+    if (s != NVQ_OK) return s;
+    char* ws = (char*)d_workspace;
+    float2* partial = (float2*)ws;
+    float* logit = (float*)(ws + sp.partial);
+    float2* block_sum = (float2*)(ws + sp.partial + sp.logit);
+    CeParams p = {};
+    p.M = (int)M;
+    p.N = (int)V;
+    p.K = (int)K;
+    p.splits = 1;
+    p.f16 = dtype == NVQ_F16;
+    p.bias = d_bias;
+    p.labels = d_labels;
+    p.partial = partial;
+    p.label_logit = logit;
+    s = launch_gemm<kLse, false, false>(p, a, b, device, st);
+    if (s != NVQ_OK) return s;
+    const int blocks = (int)((M + 31) / 32), slots = 2 * p.n_blocks;
+    s = launch_after(join_lse_kernel, blocks, JOIN_WARPS * 32, 0, st, d_row_stats, d_row_loss, block_sum, partial, logit,
+                     d_labels, (int)M, slots, (int)V, ignore_index, p.status);
+    if (s != NVQ_OK) return s;
+    return launch_after(loss_kernel, 1, 256, 0, st, d_loss_count, block_sum, blocks,
+                        (int)(reduction == NVQ_REDUCE_MEAN));
+}
+
+extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_dtype, float* d_db, const void* d_x,
+                                        const void* d_w, nvq_dtype dtype, const float* d_bias, const int32_t* d_labels,
+                                        const float* d_row_stats, const float* d_loss_count, float grad_scale, size_t M,
+                                        size_t V, size_t K, int32_t ignore_index, int reduction, void* d_workspace,
+                                        size_t workspace_bytes, int device, void* stream) {
+    nvq_status s = check_shape("nvq_linear_ce_bwd", d_x, d_w, dtype, d_bias, d_labels, M, V, K, reduction);
+    if (s != NVQ_OK) return s;
+    NVQ_REQUIRE(grad_dtype == NVQ_F32 || grad_dtype == dtype,
+                "nvq_linear_ce_bwd: gradients are f32 or of the operands' type, not %d", (int)grad_dtype);
+    NVQ_REQUIRE(nvq_aligned(d_dx, 16) && nvq_aligned(d_dw, 16) && nvq_aligned(d_db, 4),
+                "nvq_linear_ce_bwd: dx and dw must be 16-byte aligned");
+    NVQ_REQUIRE(M == 0 || (d_row_stats && d_loss_count && nvq_aligned(d_row_stats, 4) && nvq_aligned(d_loss_count, 4)),
+                "nvq_linear_ce_bwd: needs the row statistics, loss and count that nvq_linear_ce_fwd left");
+    const size_t size = grad_dtype == NVQ_F32 ? 4 : 2;
+    BwdSpace sp = {};
+    if (M) sp = bwd_space(M, V, K, kDefaultPairs);
+    NVQ_REQUIRE(M == 0 || (d_workspace && workspace_bytes >= sp.total && nvq_aligned(d_workspace, 256)),
+                "nvq_linear_ce_bwd: workspace of %zu bytes (256-byte aligned) required", sp.total);
+    s = nvq_use_device(device);
+    if (s != NVQ_OK) return s;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (M == 0) {
+        if (d_dw) NVQ_CUDA(cudaMemsetAsync(d_dw, 0, V * K * size, st));
+        if (d_db) NVQ_CUDA(cudaMemsetAsync(d_db, 0, V * sizeof(float), st));
+        return NVQ_OK;
+    }
+    if (!d_dx && !d_dw && !d_db) return NVQ_OK;
+    char* ws = (char*)d_workspace;
+    uint16_t* prob = (uint16_t*)ws;
+    float* cols = (float*)(ws + sp.prob);
+    float* sum = (float*)(ws + sp.prob + sp.cols);
+    float* parts = (float*)(ws + sp.prob + sp.cols + sp.sum);
+    const float* count = reduction == NVQ_REDUCE_MEAN ? d_loss_count + 1 : nullptr;
+    const float gain = dtype == NVQ_F16 ? F16_GAIN : 1.f;
+    const size_t piece = piece_of(M, V);
+    CUtensorMap x_k, x_mn;      // X with the contraction along its rows, and across them
+    s = nvq_make_tmap_2d(&x_k, d_x, M, K, 128, BK, 2, 1);
+    if (s != NVQ_OK) return s;
+    s = nvq_make_tmap_2d(&x_mn, d_x, M, K, BK, 64, 2, 1);
+    if (s != NVQ_OK) return s;
+    for (size_t v0 = 0; v0 < V; v0 += piece) {
+        const size_t nv = V - v0 < piece ? V - v0 : piece, ld = (nv + 15) / 16 * 16;
+        const uint16_t* w = (const uint16_t*)d_w + v0 * K;
+        CUtensorMap w_k, w_mn, g_k, g_mn;
+        if ((s = nvq_make_tmap_2d(&w_k, w, nv, K, 64, BK, 2, 1)) != NVQ_OK) return s;
+        if ((s = nvq_make_tmap_2d(&w_mn, w, nv, K, BK, 64, 2, 1)) != NVQ_OK) return s;
+        if ((s = nvq_make_tmap_2d(&g_k, prob, M, ld, 128, BK, 2, 1)) != NVQ_OK) return s;
+        if ((s = nvq_make_tmap_2d(&g_mn, prob, M, ld, BK, 64, 2, 1)) != NVQ_OK) return s;
+        CeParams p = {};
+        p.M = (int)M;
+        p.N = (int)nv;
+        p.K = (int)K;
+        p.splits = 1;
+        p.f16 = dtype == NVQ_F16;
+        p.bias = d_bias ? d_bias + v0 : nullptr;
+        p.labels = d_labels;
+        p.stats = d_row_stats;
+        p.v0 = (int)v0;
+        p.vocab = (int)V;
+        p.ignore = ignore_index;
+        p.prob = prob;
+        p.ldp = (int)ld;
+        p.col_partial = d_db ? cols : nullptr;
+        s = launch_gemm<kProb, false, false>(p, x_k, w_k, device, st);
+        if (s != NVQ_OK) return s;
+        if (d_db) {
+            s = launch_after(bias_grad_kernel, (nv + 31) / 32, 256, 0, st, d_db + v0, cols, (int)((M + 31) / 32),
+                             (int)ld, (int)nv, grad_scale, count);
+            if (s != NVQ_OK) return s;
+        }
+        if (d_dx) {
+            const bool last = v0 + nv == V;
+            CeParams q = {};
+            q.M = (int)M;
+            q.N = (int)K;
+            q.K = (int)nv;
+            q.f16 = p.f16;
+            q.add = v0 ? sum : nullptr;
+            q.sum = last ? nullptr : sum;
+            q.out = last ? d_dx : nullptr;
+            q.out_type = grad_dtype;
+            q.vec32 = K * size % 32 == 0 && nvq_aligned(d_dx, 32);
+            q.scale = grad_scale / gain;
+            q.count = count;
+            s = contract<false, true>(q, g_k, w_mn, parts, device, st);
+            if (s != NVQ_OK) return s;
+        }
+        if (d_dw) {
+            CeParams q = {};
+            q.M = (int)nv;
+            q.N = (int)K;
+            q.K = (int)M;
+            q.f16 = p.f16;
+            q.out = (char*)d_dw + v0 * K * size;
+            q.out_type = grad_dtype;
+            q.vec32 = K * size % 32 == 0 && nvq_aligned(d_dw, 32);
+            q.scale = grad_scale / gain;
+            q.count = count;
+            s = contract<true, true>(q, g_mn, x_mn, parts, device, st);
+            if (s != NVQ_OK) return s;
+        }
+    }
+    return NVQ_OK;
+}

@@ -81,6 +81,17 @@ template <int DT, int V> struct Packet {
             load(p);
         }
     }
+    // the same for memory that this kernel may write (in place)
+    __device__ __forceinline__ void load_once(const void* p) {
+        if constexpr (BYTES == 16) {
+            asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "l"(p)
+                         : "memory");
+        } else {
+            load(p);
+        }
+    }
     __device__ __forceinline__ void store(void* p) const {
         if constexpr (BYTES == 16) stg_stream_128(p, make_uint4(w[0], w[1], w[2], w[3]));
         else if constexpr (BYTES == 4) *(uint32_t*)p = w[0];

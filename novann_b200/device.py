@@ -148,8 +148,12 @@ class DeviceBuffer:
 class DeviceView:
     """Device memory owned by someone else, with ``DeviceBuffer``'s addressing."""
 
+    __slots__ = ("ptr", "nbytes", "device")
+
     def __init__(self, ptr: int, nbytes: int, device: int = 0):
-        self.ptr, self.nbytes, self.device = ptr, nbytes, device
+        self.ptr = ptr
+        self.nbytes = nbytes
+        self.device = device
 
     def at(self, offset: int) -> C.c_void_p:
         return C.c_void_p(self.ptr + offset)

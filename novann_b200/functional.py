@@ -7,6 +7,8 @@ returns NumPy arrays (bf16 as uint16 bit patterns).
 from __future__ import annotations
 
 import ctypes as C
+from array import array
+from itertools import repeat
 
 import numpy as np
 
@@ -587,8 +589,8 @@ def embedding_device(out: DeviceBuffer, table: DeviceBuffer, dtype: str, ids: De
     _holds("out", out, t * d * size)
     _holds("table", table, v * d * size)
     _holds("ids", ids, t * 4)
-    check(lib().nvq_embedding_fwd(out.at(0), table.at(0), _lib.DTYPE_IDS[dtype], ids.at(0), t, v, d,
-                                  C.c_float(scale), table.device, _sptr(stream)))
+    check(lib().nvq_embedding_fwd(out.ptr, table.ptr, _lib.DTYPE_IDS[dtype], ids.ptr, t, v, d, scale, table.device,
+                                  _sptr(stream)))
 
 
 def embedding_bwd_workspace_bytes(t: int, v: int, d: int) -> int:
@@ -607,9 +609,9 @@ def embedding_bwd_device(dtable: DeviceBuffer, dout: DeviceBuffer, dtype: str, i
     _holds("dtable", dtable, v * d * 4)
     _holds("dout", dout, t * d * size)
     _holds("ids", ids, t * 4)
-    check(lib().nvq_embedding_bwd(dtable.at(0), dout.at(0), _lib.DTYPE_IDS[dtype], ids.at(0), t, v, d,
-                                  C.c_float(scale), -1 if padding_id is None else padding_id, int(accumulate),
-                                  workspace.at(0), workspace.nbytes, dtable.device, _sptr(stream)))
+    check(lib().nvq_embedding_bwd(dtable.ptr, dout.ptr, _lib.DTYPE_IDS[dtype], ids.ptr, t, v, d, scale,
+                                  -1 if padding_id is None else padding_id, int(accumulate), workspace.ptr,
+                                  workspace.nbytes, dtable.device, _sptr(stream)))
 
 
 def _host_ids(ids, v: int) -> np.ndarray:
@@ -659,6 +661,112 @@ def embedding_bwd_host(dout, ids, v: int, scale: float = 1.0, padding_id: int | 
     return o.to_numpy(np.float32, (v, d))
 
 
+# ------------------------------------------------------------------ linear + softmax cross entropy
+_HALVES = {"f16": 2, "bf16": 2}
+
+
+def _reduction(name: str) -> int:
+    if name not in _lib.REDUCTIONS:
+        raise ValueError(f"reduction must be one of {tuple(_lib.REDUCTIONS)}, not {name!r}")
+    return _lib.REDUCTIONS[name]
+
+
+def linear_ce_workspace_bytes(m: int, v: int, k: int, backward: bool = True) -> int:
+    out = C.c_size_t()
+    check(lib().nvq_linear_ce_workspace_bytes(m, v, k, int(backward), C.byref(out)))
+    return out.value
+
+
+def linear_ce_device(loss: DeviceBuffer, stats: DeviceBuffer, x: DeviceBuffer, w: DeviceBuffer, dtype: str,
+                     labels: DeviceBuffer, m: int, v: int, k: int, workspace: DeviceBuffer,
+                     bias: DeviceBuffer | None = None, row_loss: DeviceBuffer | None = None, ignore_index: int = -100,
+                     reduction: str = "mean", stream=None) -> None:
+    """Softmax cross entropy of ``x @ w.T + bias`` against int32 labels, the (m, v) logits never kept:
+    x (m, k) and w (v, k) "f16" or "bf16", k a multiple of 8, bias (v,) fp32.  Writes loss (2 floats: the
+    sum or mean over the rows whose label is not ``ignore_index``, and their number), row_loss (m,) and
+    stats (2, m) fp32: the rows' largest logits and the logarithms of their sums of exp(logit - largest)."""
+    _float_type(dtype, _HALVES)
+    _holds("loss", loss, 8)
+    _holds("stats", stats, m * 8)
+    _holds("x", x, m * k * 2)
+    _holds("w", w, v * k * 2)
+    _holds("labels", labels, m * 4)
+    if bias is not None:
+        _holds("bias", bias, v * 4)
+    if row_loss is not None:
+        _holds("row_loss", row_loss, m * 4)
+    check(lib().nvq_linear_ce_fwd(loss.ptr, row_loss.ptr if row_loss is not None else None, stats.ptr, x.ptr, w.ptr,
+                                  _lib.DTYPE_IDS[dtype], bias.ptr if bias is not None else None, labels.ptr, m, v, k,
+                                  ignore_index, _reduction(reduction), workspace.ptr, workspace.nbytes, w.device,
+                                  _sptr(stream)))
+
+
+def linear_ce_bwd_device(dx: DeviceBuffer | None, dw: DeviceBuffer | None, x: DeviceBuffer, w: DeviceBuffer,
+                         dtype: str, labels: DeviceBuffer, stats: DeviceBuffer, loss: DeviceBuffer, m: int, v: int,
+                         k: int, workspace: DeviceBuffer, bias: DeviceBuffer | None = None,
+                         db: DeviceBuffer | None = None, grad_dtype: str = "f32", grad_scale: float = 1.0,
+                         ignore_index: int = -100, reduction: str = "mean", stream=None) -> None:
+    """Gradients of ``grad_scale * loss`` from the ``stats`` and ``loss`` that ``linear_ce_device`` left:
+    dx (m, k) and dw (v, k) as ``grad_dtype`` ("f32" or the operands' type), db (v,) fp32; None skips one.
+    The logits are computed again, a piece of the vocabulary at a time."""
+    _float_type(dtype, _HALVES)
+    if grad_dtype not in ("f32", dtype):
+        raise ValueError(f"grad_dtype must be 'f32' or {dtype!r}, not {grad_dtype!r}")
+    size = _FLOATS[grad_dtype]
+    _holds("x", x, m * k * 2)
+    _holds("w", w, v * k * 2)
+    _holds("labels", labels, m * 4)
+    _holds("stats", stats, m * 8)
+    _holds("loss", loss, 8)
+    for name, buf, nbytes in (("dx", dx, m * k * size), ("dw", dw, v * k * size), ("db", db, v * 4),
+                              ("bias", bias, v * 4)):
+        if buf is not None:
+            _holds(name, buf, nbytes)
+    check(lib().nvq_linear_ce_bwd(dx.ptr if dx is not None else None, dw.ptr if dw is not None else None,
+                                  _lib.DTYPE_IDS[grad_dtype], db.ptr if db is not None else None, x.ptr, w.ptr,
+                                  _lib.DTYPE_IDS[dtype], bias.ptr if bias is not None else None, labels.ptr, stats.ptr,
+                                  loss.ptr, grad_scale, m, v, k, ignore_index, _reduction(reduction), workspace.ptr,
+                                  workspace.nbytes, w.device, _sptr(stream)))
+
+
+def linear_ce_host(x, w, labels, bias=None, ignore_index: int = -100, reduction: str = "mean", grad: bool = True,
+                   grad_scale: float = 1.0, device: int = 0):
+    """``linear_ce_device`` and its gradients for host arrays: x (M, K) and w (V, K) float16, or bf16 bits
+    (uint16).  Returns (loss, row_loss) and, with ``grad``, (loss, row_loss, dx, dw, db) in float32 (db
+    None without a bias)."""
+    x, dtype = _host_float(x)
+    w, wt = _host_float(w)
+    if dtype not in _HALVES or wt != dtype:
+        raise TypeError("x and w must both be float16 or both bf16 bits (uint16)")
+    (m, k), v = x.shape, w.shape[0]
+    if w.shape[1] != k:
+        raise ValueError(f"x has {k} features, w {w.shape[1]}")
+    labels = np.asarray(labels)
+    if labels.shape != (m,) or labels.dtype.kind not in "iu":
+        raise ValueError(f"labels must be {m} integers")
+    kept = labels[labels != ignore_index]
+    if kept.size and (int(kept.min()) < 0 or int(kept.max()) >= v):
+        raise IndexError(f"label out of range for {v} classes")
+    dx_, dw_ = DeviceBuffer.from_numpy(x, device), DeviceBuffer.from_numpy(w, device)
+    dl = DeviceBuffer.from_numpy(labels.astype(np.int32), device)
+    db_ = None if bias is None else DeviceBuffer.from_numpy(_f32(bias, device).reshape(-1), device)
+    ws = DeviceBuffer(linear_ce_workspace_bytes(m, v, k, grad), device)
+    head, stats, rows = DeviceBuffer(8, device), DeviceBuffer(m * 8, device), DeviceBuffer(m * 4, device)
+    linear_ce_device(head, stats, dx_, dw_, dtype, dl, m, v, k, ws, db_, rows, ignore_index, reduction)
+    if grad:
+        o_dx, o_dw = DeviceBuffer(m * k * 4, device), DeviceBuffer(v * k * 4, device)
+        o_db = None if bias is None else DeviceBuffer(v * 4, device)
+        linear_ce_bwd_device(o_dx, o_dw, dx_, dw_, dtype, dl, stats, head, m, v, k, ws, db_, o_db, "f32", grad_scale,
+                             ignore_index, reduction)
+    device_sync(device)
+    check_device_errors(device)
+    out = (head.to_numpy(np.float32, (2,))[0], rows.to_numpy(np.float32, (m,)))
+    if grad:
+        out += (o_dx.to_numpy(np.float32, (m, k)), o_dw.to_numpy(np.float32, (v, k)),
+                None if o_db is None else o_db.to_numpy(np.float32, (v,)))
+    return out
+
+
 # ------------------------------------------------------------------ gradient norm and clipping
 _GRADS = {**_FLOATS, "f64": 8}
 
@@ -670,20 +778,24 @@ def grad_norm_workspace_bytes() -> int:
 
 
 def _tensor_list(what: str, bufs, counts, dtypes):
+    """Host arrays of pointers, counts and type ids of a list of tensors."""
     n = len(bufs)
-    if len(counts) != n or (not isinstance(dtypes, str) and len(dtypes) != n):
+    one = isinstance(dtypes, str)
+    if len(counts) != n or (not one and len(dtypes) != n):
         raise ValueError("tensors, counts and dtypes must be of one length")
-    names = [dtypes] * n if isinstance(dtypes, str) else dtypes
-    sizes = [_float_type(name, _GRADS) for name in names]
-    ptrs = []
+    sizes = repeat(_float_type(dtypes, _GRADS)) if one else [_float_type(name, _GRADS) for name in dtypes]
     for b, count, size in zip(bufs, counts, sizes):
         if count < 0 or b.nbytes < count * size:
             raise ValueError(f"{what}: a buffer of {b.nbytes} bytes does not hold {count} elements")
-        ptrs.append(b.ptr)
+    ptrs = [b.ptr for b in bufs]
     if len(set(ptrs)) != n and len({p for p, c in zip(ptrs, counts) if c}) != sum(1 for c in counts if c):
         raise ValueError(f"{what}: a tensor is listed twice")
-    return ((C.c_void_p * n)(*ptrs), (C.c_size_t * n)(*counts),
-            (C.c_int32 * n)(*[_lib.DTYPE_IDS[name] for name in names]), n)
+    types = array("i", [_lib.DTYPE_IDS[dtypes]]) * n if one else array("i", [_lib.DTYPE_IDS[x] for x in dtypes])
+    return array("Q", ptrs), array("Q", counts), types
+
+
+def _address(a) -> int:
+    return a.buffer_info()[0]
 
 
 def grad_norm_device(norm: DeviceBuffer, grads, counts, dtypes, workspace: DeviceBuffer,
@@ -692,19 +804,20 @@ def grad_norm_device(norm: DeviceBuffer, grads, counts, dtypes, workspace: Devic
     ``max_norm`` would apply.  ``grads``: device buffers, ``counts``: their elements, ``dtypes``: one
     name for all or one each ("f32", "f16", "bf16", "f64")."""
     _holds("norm", norm, 8)
-    ptrs, n_el, types, n = _tensor_list("grads", grads, counts, dtypes)
-    check(lib().nvq_grad_norm(norm.at(0), ptrs, n_el, types, n, float(max_norm), workspace.at(0), workspace.nbytes,
-                              norm.device, _sptr(stream)))
+    ptrs, n_el, types = _tensor_list("grads", grads, counts, dtypes)
+    check(lib().nvq_grad_norm(norm.ptr, _address(ptrs), _address(n_el), _address(types), len(ptrs), max_norm,
+                              workspace.ptr, workspace.nbytes, norm.device, _sptr(stream)))
 
 
 def clip_grads_device(norm: DeviceBuffer, grads, counts, dtypes, max_norm: float, workspace: DeviceBuffer, out=None,
                       stream=None) -> None:
     """``grad_norm_device``, then every gradient times the factor: in place, or into ``out``."""
     _holds("norm", norm, 8)
-    ptrs, n_el, types, n = _tensor_list("grads", grads, counts, dtypes)
+    ptrs, n_el, types = _tensor_list("grads", grads, counts, dtypes)
     to = None if out is None else _tensor_list("out", out, counts, dtypes)[0]
-    check(lib().nvq_clip_grads(norm.at(0), to, ptrs, n_el, types, n, float(max_norm), workspace.at(0),
-                               workspace.nbytes, norm.device, _sptr(stream)))
+    check(lib().nvq_clip_grads(norm.ptr, None if to is None else _address(to), _address(ptrs), _address(n_el),
+                               _address(types), len(ptrs), max_norm, workspace.ptr, workspace.nbytes, norm.device,
+                               _sptr(stream)))
 
 
 def clip_grad_norm(parameters, max_norm: float, device: int = 0) -> np.float32:

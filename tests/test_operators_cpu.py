@@ -102,3 +102,55 @@ def test_optimiser_and_step_refusals():
         MLPTrainStep([], 4, 0.1, max_grad_norm=0.0)
     with pytest.raises(ValueError, match="peer"):
         MLPTrainStep([], 4, 0.1, peer=object(), max_grad_norm=1.0)
+
+
+def test_linear_ce_refusals():
+    L = _lib.lib()
+    need = F.linear_ce_workspace_bytes(100, 50, 16)
+
+    def fwd(dtype=_lib.BF16, m=100, v=50, k=16, x=P, w=P, labels=P, loss=P, stats=P, red=1, ws=P, nbytes=need):
+        return L.nvq_linear_ce_fwd(loss, None, stats, x, w, dtype, None, labels, m, v, k, -100, red, ws, nbytes, 0, None)
+
+    def bwd(dtype=_lib.BF16, grad=_lib.F32, dx=P, dw=P, stats=P, loss=P, ws=P, nbytes=need, k=16):
+        return L.nvq_linear_ce_bwd(dx, dw, grad, None, P, P, dtype, None, P, stats, loss, 1.0, 100, 50, k, -100, 1, ws,
+                                   nbytes, 0, None)
+    refused(fwd(dtype=_lib.F32), "type")
+    refused(fwd(k=12), "multiple of 8")
+    refused(fwd(v=0), "V in")
+    refused(fwd(red=2), "reduction")
+    refused(fwd(x=None), "aligned")
+    refused(fwd(w=C.c_void_p(264)), "aligned")
+    refused(fwd(labels=None), "labels")
+    refused(fwd(stats=None), "output")
+    refused(fwd(loss=None), "output")
+    refused(fwd(nbytes=16), "workspace")
+    refused(fwd(ws=C.c_void_p(128)), "workspace")
+    refused(bwd(grad=_lib.F16), "gradients")
+    refused(bwd(dx=C.c_void_p(264)), "aligned")
+    refused(bwd(stats=None), "statistics")
+    refused(bwd(nbytes=need - 1), "workspace", str(need))
+    refused(bwd(k=4), "multiple of 8")
+    v = DeviceView(256, 64)
+    with pytest.raises(ValueError, match="reduction"):
+        F.linear_ce_device(v, v, v, v, "bf16", v, 1, 1, 8, v, reduction="none")
+    with pytest.raises(ValueError, match="hold"):
+        F.linear_ce_device(v, v, v, v, "bf16", v, 1, 5, 8, v)
+    with pytest.raises(ValueError, match="grad_dtype"):
+        F.linear_ce_bwd_device(v, v, v, v, "bf16", v, v, v, 1, 1, 8, v, grad_dtype="f16")
+    x, w = np.zeros((2, 16), np.float16), np.zeros((5, 16), np.float16)
+    with pytest.raises(IndexError):
+        F.linear_ce_host(x, w, np.array([0, 5]))
+    with pytest.raises(ValueError, match="labels"):
+        F.linear_ce_host(x, w, np.array([0]))
+    with pytest.raises(TypeError):
+        F.linear_ce_host(x, w.view(np.uint16), np.array([0, 1]))
+    with pytest.raises(ValueError, match="features"):
+        F.linear_ce_host(x, w[:, :8], np.array([0, 1]))
+    with pytest.raises(ValueError, match="multiple of 8"):
+        nb.LinearCrossEntropyLoss(12, 5)
+    with pytest.raises(ValueError, match="dtype"):
+        nb.LinearCrossEntropyLoss(16, 5, dtype="f32")
+    head = nb.LinearCrossEntropyLoss(16, 5, bias=False)
+    assert len(head.parameters()) == 1
+    with pytest.raises(RuntimeError):
+        head.backward()
