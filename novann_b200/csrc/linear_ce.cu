@@ -14,6 +14,8 @@
 //   kSum   fp32 sums: added to a buffer, or scaled and rounded to the gradient's type
 // The backward pass computes the logits of a piece a second time instead of keeping M x V of them:
 // 8 M V K operations where 6 M V K are needed, against reading and writing the logits twice.
+#include <type_traits>
+
 #include "gemm_common.cuh"
 #include "packet.cuh"
 
@@ -34,10 +36,22 @@ constexpr float F16_GAIN = 16384.f;
 enum { kLse = 0, kProb = 1, kSum = 2 };
 enum { ERR_PRODUCER = 81, ERR_MMA_FULL = 82, ERR_MMA_TMEM = 83, ERR_EPILOGUE = 84, ERR_LABEL = 85 };
 
-struct CeParams : LinearParams {
+// One contraction: (M x K) times (K x N) in 256 x 256 tiles
+struct Problem : LinearParams {
     int splits, kb_per;          // the contraction cut into `splits` parts of kb_per k-blocks
+    int a_mn;                    // kSum: A is stored with M contiguous instead of the contraction
+    const float* add;            // fp32 sums of earlier pieces (M x N), or nullptr
+    float* sum;                  // where fp32 sums go (M x N each; split s at s * M * N), or nullptr
+    void* out;                   // final result, or nullptr
+    int vec32;                   // out's rows start on 32-byte boundaries
+};
+
+struct CeParams {
+    Problem q[2];                // kSum: up to two contractions in one launch, the longer items first
     int f16;                     // operands are fp16 (else bf16)
+    int* status;
     // kLse, kProb
+    const float* bias;
     const int32_t* labels;
     float2* partial;             // kLse: (2 * n_blocks) x M maxima and sums
     float* label_logit;          // kLse: M
@@ -45,15 +59,14 @@ struct CeParams : LinearParams {
     int v0, vocab, ignore;       // kProb: first vocabulary entry of this piece, vocabulary, label that does not count
     uint16_t* prob;              // kProb: M x ldp, ldp a multiple of 16, 0 past the piece
     int ldp;
-    float* col_partial;          // kProb: ceil(M / 32) x ldp column sums of 32 rows each, or nullptr
+    float* col_partial;          // ceil(M / 32) x ldp column sums of 32 rows each (kProb writes, kSum adds up), or nullptr
     // kSum
-    const float* add;            // fp32 sums of earlier pieces (M x N), or nullptr
-    float* sum;                  // where fp32 sums go (M x N each; split s at s * M * N), or nullptr
-    void* out;                   // final result in out_type, or nullptr
     int out_type;
-    int vec32;                   // out's rows start on 32-byte boundaries
-    float scale;                 // factor of the final result, over the count of rows where `count` is set
+    float scale;                 // factor of the final results, over the count of rows where `count` is set
     const float* count;
+    float* db;                   // the column sums' sums, db_n of them over `groups` groups of rows, times db_scale
+    int db_n, groups;
+    float db_scale;
 };
 
 struct Shared {
@@ -64,6 +77,7 @@ struct Shared {
     uint32_t tmem_base;
     int abort_flag;
     alignas(16) float bias[2][BN];
+    float db_part[EPI_WARPS][32];
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -85,25 +99,35 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
     return d;
 }
 
-struct Item { TileRef tile; int kb0, kb1, split; };
-__device__ __forceinline__ Item item_of(const CeParams& p, int t, int num_kb) {
+struct Item { const Problem* q; TileRef tile; int kb0, kb1, split; bool second; };
+__device__ __forceinline__ Item item_of(const CeParams& p, int t) {
     Item it;
+    it.second = t >= p.q[0].num_items;
+    it.q = &p.q[it.second];
+    if (it.second) t -= p.q[0].num_items;
     it.split = 0;
     it.kb0 = 0;
-    it.kb1 = num_kb;
-    if (p.splits > 1) {          // num_items = tiles * splits, a tile's parts next to one another
-        it.split = t % p.splits;
-        t /= p.splits;
-        it.kb0 = it.split * p.kb_per;
-        it.kb1 = min(num_kb, it.kb0 + p.kb_per);
+    it.kb1 = (it.q->K + BK - 1) / BK;
+    if (it.q->splits > 1) {          // num_items = tiles * splits, a tile's parts next to one another
+        it.split = t % it.q->splits;
+        t /= it.q->splits;
+        it.kb0 = it.split * it.q->kb_per;
+        it.kb1 = min(it.kb1, it.kb0 + it.q->kb_per);
     }
-    it.tile = tile_ref(p, t);
+    it.tile = tile_ref(*it.q, t);
     return it;
 }
 
+// kLse keeps at most this many k-blocks (1024 of K) in one TMEM accumulator: the tensor core cuts off where it adds, by
+// up to a step of the running sum each time, and over 4096 of K the logits were off by 1e-6 of themselves, all
+// towards zero.  The parts are joined in registers; MMAs and epilogue alternate between the two accumulators as
+// they do between tiles.
+constexpr int PART_KB = 16;
+
 // 32 fp32 sums of one row (columns n ...): to the fp32 buffer, or scaled to the final type
-__device__ __forceinline__ void store_sum(const CeParams& p, const uint32_t* r, size_t at, int n, int split, float s) {
-    if (p.out == nullptr || p.out_type == NVQ_F32) {
+__device__ __forceinline__ void store_sum(const Problem& p, int out_type, const uint32_t* r, size_t at, int n, int split,
+                                          float s) {
+    if (p.out == nullptr || out_type == NVQ_F32) {
         float* dst = p.out ? (float*)p.out + at : p.sum + (size_t)split * p.M * p.N + at;
         const bool wide = p.out == nullptr || p.vec32;
 #pragma unroll
@@ -128,7 +152,7 @@ __device__ __forceinline__ void store_sum(const CeParams& p, const uint32_t* r, 
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float a = __uint_as_float(r[g + 2 * j]) * s, b = __uint_as_float(r[g + 2 * j + 1]) * s;
-                o.v[j] = p.out_type == NVQ_F16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+                o.v[j] = out_type == NVQ_F16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
             }
             if (p.vec32 && n + g + 16 <= p.N) {
                 stg_stream_256(dst + g, o);
@@ -140,11 +164,13 @@ __device__ __forceinline__ void store_sum(const CeParams& p, const uint32_t* r, 
     }
 }
 
-// A_MN / B_MN: the operand is stored with its own dimension contiguous instead of the contraction's
-template <int EPI, bool A_MN, bool B_MN>
+// kLse, kProb: both operands with the contraction contiguous.  kSum: B with N contiguous, A as Problem::a_mn says.
+template <int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-               const CeParams p) {
+ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
+               const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
+               const __grid_constant__ CeParams p) {
+    constexpr bool B_MN = EPI == kSum;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = tc::smem_u32(smem_raw);
     const uint32_t tiles = (raw + 1023u) & ~1023u;
@@ -152,29 +178,29 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_ctarank();
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-    const int num_kb = (p.K + BK - 1) / BK;
+    const int num_items = p.q[0].num_items + p.q[1].num_items;
     volatile int* abort_flag = &sh->abort_flag;
-    // accumulators: two of 256 columns, or four of 128 when the output has at most 128 columns
-    const bool narrow = p.N <= BN / 2;
-    const uint32_t acc_cols = narrow ? BN / 2 : BN;
-    auto acc_of = [&](int it, uint32_t& acc, uint32_t& acc_phase) {
-        if (narrow) { acc = it & 3; acc_phase = (it >> 2) & 1; }
-        else        { acc = it & 1; acc_phase = (it >> 1) & 1; }
-    };
+    // accumulators: two of 256 columns
+    auto acc_of = [&](int n, uint32_t& acc, uint32_t& acc_phase) { acc = n & 1; acc_phase = (n >> 1) & 1; };
+    const int part_kb = EPI == kLse ? PART_KB : 1 << 30;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
             tc::mbar_init(tc::smem_u32(&sh->full[s]), 1);
             tc::mbar_init(tc::smem_u32(&sh->empty[s]), 1);
         }
-        for (int a = 0; a < 4; a++) {
+        for (int a = 0; a < 2; a++) {
             tc::mbar_init(tc::smem_u32(&sh->tmem_full[a]), 1);
             tc::mbar_init(tc::smem_u32(&sh->tmem_empty[a]), 2 * EPI_WARPS);
         }
         sh->abort_flag = 0;
         tc::mbar_fence_init();
-        tc::tma_prefetch_desc(&map_a);
-        tc::tma_prefetch_desc(&map_b);
+        tc::tma_prefetch_desc(&map_a0);
+        tc::tma_prefetch_desc(&map_b0);
+        if (EPI == kSum) {
+            tc::tma_prefetch_desc(&map_a1);
+            tc::tma_prefetch_desc(&map_b1);
+        }
     }
     if (warp == 1) {
         tc::tmem_alloc_pair(tc::smem_u32(&sh->tmem_base), TMEM_COLS);
@@ -192,8 +218,10 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (int t = pair; t < p.num_items && ok; t += num_pairs) {
-                const Item it = item_of(p, t, num_kb);
+            for (int t = pair; t < num_items && ok; t += num_pairs) {
+                const Item it = item_of(p, t);
+                const CUtensorMap* map_a = it.second ? &map_a1 : &map_a0;
+                const CUtensorMap* map_b = it.second ? &map_b1 : &map_b0;
                 const int rows_b = it.tile.is_half ? BN / 4 : BN / 2;       // per CTA
                 const int m0 = it.tile.m_blk * BM + (int)rank * 128;
                 const int n0 = it.tile.n_blk * BN + it.tile.half * (BN / 2) + (int)rank * rows_b;
@@ -204,20 +232,20 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     const uint32_t lead_full = tc::mapa(tc::smem_u32(&sh->full[stage]), 0);
                     if (rank == 0)       // the leader expects the bytes of both CTAs
                         tc::mbar_arrive_expect_tx(tc::smem_u32(&sh->full[stage]), 2 * (A_BYTES + rows_b * BK * 2));
-                    if constexpr (A_MN) {
-                        tc::tma_load_2d_pair(dst, &map_a, lead_full, m0, kb * BK);
-                        tc::tma_load_2d_pair(dst + A_BYTES / 2, &map_a, lead_full, m0 + 64, kb * BK);
+                    if (EPI == kSum && it.q->a_mn) {
+                        tc::tma_load_2d_pair(dst, map_a, lead_full, m0, kb * BK);
+                        tc::tma_load_2d_pair(dst + A_BYTES / 2, map_a, lead_full, m0 + 64, kb * BK);
                     } else {
-                        tc::tma_load_2d_pair(dst, &map_a, lead_full, kb * BK, m0);
+                        tc::tma_load_2d_pair(dst, map_a, lead_full, kb * BK, m0);
                     }
                     if constexpr (B_MN) {
-                        tc::tma_load_2d_pair(dst + A_BYTES, &map_b, lead_full, n0, kb * BK);
+                        tc::tma_load_2d_pair(dst + A_BYTES, map_b, lead_full, n0, kb * BK);
                         if (rows_b == 128)
-                            tc::tma_load_2d_pair(dst + A_BYTES + B_BYTES / 2, &map_b, lead_full, n0 + 64, kb * BK);
+                            tc::tma_load_2d_pair(dst + A_BYTES + B_BYTES / 2, map_b, lead_full, n0 + 64, kb * BK);
                     } else {
-                        tc::tma_load_2d_pair(dst + A_BYTES, &map_b, lead_full, kb * BK, n0);
+                        tc::tma_load_2d_pair(dst + A_BYTES, map_b, lead_full, kb * BK, n0);
                         if (rows_b == 128)
-                            tc::tma_load_2d_pair(dst + A_BYTES + B_BYTES / 2, &map_b, lead_full, kb * BK, n0 + 64);
+                            tc::tma_load_2d_pair(dst + A_BYTES + B_BYTES / 2, map_b, lead_full, kb * BK, n0 + 64);
                     }
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
@@ -230,40 +258,45 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             bool ok = true, ready = false;
             int n = 0;
             const uint32_t fmt = p.f16 ? 0u : 1u;
-            const uint32_t major = (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
-            for (int t = pair; t < p.num_items && ok; t += num_pairs, n++) {
-                uint32_t acc, acc_phase;
-                acc_of(n, acc, acc_phase);
-                const Item it = item_of(p, t, num_kb);
-                const uint32_t idesc = tc::idesc_f16(BM, it.tile.is_half ? BN / 2 : BN, fmt, fmt) | major;
-                ok = tc::mbar_wait(tc::smem_u32(&sh->tmem_empty[acc]), acc_phase ^ 1, abort_flag, ERR_MMA_TMEM);
-                if (!ok) break;
-                tc::tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * acc_cols;
-                for (int kb = it.kb0; kb < it.kb1; kb++) {
-                    if (!ready) {
-                        ok = tc::mbar_wait(tc::smem_u32(&sh->full[stage]), phase, abort_flag, ERR_MMA_FULL);
-                        if (!ok) break;
-                    }
+            for (int t = pair; t < num_items && ok; t += num_pairs) {
+                const Item it = item_of(p, t);
+                const bool a_mn = EPI == kSum && it.q->a_mn;
+                const uint32_t idesc = tc::idesc_f16(BM, it.tile.is_half ? BN / 2 : BN, fmt, fmt) |
+                                       (a_mn ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+                // 16 contraction steps: 32 bytes along a row, or 16 rows of 128 bytes
+                const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4;
+                constexpr uint32_t b_step = B_MN ? 2048 >> 4 : 32 >> 4;
+                for (int k0 = it.kb0; k0 < it.kb1 && ok; k0 += part_kb, n++) {
+                    const int k1 = it.kb1 - k0 < part_kb ? it.kb1 : k0 + part_kb;
+                    uint32_t acc, acc_phase;
+                    acc_of(n, acc, acc_phase);
+                    ok = tc::mbar_wait(tc::smem_u32(&sh->tmem_empty[acc]), acc_phase ^ 1, abort_flag, ERR_MMA_TMEM);
+                    if (!ok) break;
                     tc::tc_fence_after();
-                    const uint32_t nstage = stage + 1 == (uint32_t)STAGES ? 0u : stage + 1;
-                    const uint32_t nphase = nstage == 0 ? phase ^ 1u : phase;
-                    const uint32_t a_addr = tiles + stage * STAGE_BYTES, b_addr = a_addr + A_BYTES;
-                    const uint64_t a_desc = A_MN ? smem_desc_mn_sw128(a_addr) : tc::smem_desc_k_sw128(a_addr);
-                    const uint64_t b_desc = B_MN ? smem_desc_mn_sw128(b_addr) : tc::smem_desc_k_sw128(b_addr);
-                    // 16 contraction steps: 32 bytes along a row, or 16 rows of 128 bytes
-                    constexpr uint32_t a_step = A_MN ? 2048 >> 4 : 32 >> 4, b_step = B_MN ? 2048 >> 4 : 32 >> 4;
+                    const uint32_t d_tmem = tmem_base + acc * BN;
+                    for (int kb = k0; kb < k1; kb++) {
+                        if (!ready) {
+                            ok = tc::mbar_wait(tc::smem_u32(&sh->full[stage]), phase, abort_flag, ERR_MMA_FULL);
+                            if (!ok) break;
+                        }
+                        tc::tc_fence_after();
+                        const uint32_t nstage = stage + 1 == (uint32_t)STAGES ? 0u : stage + 1;
+                        const uint32_t nphase = nstage == 0 ? phase ^ 1u : phase;
+                        const uint32_t a_addr = tiles + stage * STAGE_BYTES, b_addr = a_addr + A_BYTES;
+                        const uint64_t a_desc = a_mn ? smem_desc_mn_sw128(a_addr) : tc::smem_desc_k_sw128(a_addr);
+                        const uint64_t b_desc = B_MN ? smem_desc_mn_sw128(b_addr) : tc::smem_desc_k_sw128(b_addr);
 #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; k++) {
-                        tc::tc_mma_f16_pair(d_tmem, a_desc + a_step * k, b_desc + b_step * k, idesc,
-                                            kb > it.kb0 || k > 0);
-                        if (k == 0) ready = tc::mbar_test_wait(tc::smem_u32(&sh->full[nstage]), nphase);
+                        for (int k = 0; k < BK / UMMA_K; k++) {
+                            tc::tc_mma_f16_pair(d_tmem, a_desc + a_step * k, b_desc + b_step * k, idesc,
+                                                kb > k0 || k > 0);
+                            if (k == 0) ready = tc::mbar_test_wait(tc::smem_u32(&sh->full[nstage]), nphase);
+                        }
+                        tc::tc_commit_pair(tc::smem_u32(&sh->empty[stage]), 3);
+                        stage = nstage;
+                        phase = nphase;
                     }
-                    tc::tc_commit_pair(tc::smem_u32(&sh->empty[stage]), 3);
-                    stage = nstage;
-                    phase = nphase;
+                    if (ok) tc::tc_commit_pair(tc::smem_u32(&sh->tmem_full[acc]), 3);
                 }
-                if (ok) tc::tc_commit_pair(tc::smem_u32(&sh->tmem_full[acc]), 3);
             }
         }
     } else {
@@ -272,103 +305,200 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const int colgrp = (warp - 2) >> 2;           // which 128 (64) columns of the tile
         const int et = threadIdx.x - 64;              // 0 .. 255
         bool ok = true;
-        int n_it = 0;
-        for (int t = pair; t < p.num_items && ok; t += num_pairs, n_it++) {
+        int n_acc = 0;
+        // the accumulator that comes next, complete; every epilogue thread takes part, whatever its lane found
+        auto take = [&](uint32_t& taddr) -> uint32_t {
             uint32_t acc, acc_phase;
-            acc_of(n_it, acc, acc_phase);
-            const Item it = item_of(p, t, num_kb);
+            acc_of(n_acc++, acc, acc_phase);
+            ok = tc::mbar_wait(tc::smem_u32(&sh->tmem_full[acc]), acc_phase, abort_flag, ERR_EPILOGUE);
+            ok = epilogue_all<32 * EPI_WARPS>(ok);
+            tc::tc_fence_after();
+            taddr = tmem_base + acc * BN + ((uint32_t)(quarter * 32) << 16);
+            return acc;
+        };
+        auto give_back = [&](uint32_t acc) {
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive_remote(tc::mapa(tc::smem_u32(&sh->tmem_empty[acc]), 0));
+        };
+
+        if constexpr (EPI == kSum) {
+            // db, while the first tile's MMAs run: 32 columns a warp where there are few groups of rows to add up,
+            // else 32 columns a CTA
+            if (p.db) {
+                const float s_db = p.count ? p.db_scale / fmaxf(*p.count, 1.f) : p.db_scale;
+                const bool alone = p.groups <= EPI_WARPS;
+                const int wide = alone ? 32 * EPI_WARPS : 32;
+                for (int c0 = (int)blockIdx.x * wide; c0 < p.db_n; c0 += (int)gridDim.x * wide) {
+                    float s = 0.f;
+                    const int c = c0 + (alone ? (warp - 2) * 32 : 0) + lane;
+                    if (c < p.db_n)
+#pragma unroll 4
+                        for (int g = alone ? 0 : warp - 2; g < p.groups; g += alone ? 1 : EPI_WARPS)
+                            s += p.col_partial[(size_t)g * p.ldp + c];
+                    if (!alone) {
+                        sh->db_part[warp - 2][lane] = s;
+                        epilogue_all<32 * EPI_WARPS>(true);
+                        s = 0.f;
+                        if (warp == 2)
+                            for (int w = 0; w < EPI_WARPS; w++) s += sh->db_part[w][lane];
+                        epilogue_all<32 * EPI_WARPS>(true);
+                    }
+                    if (c < p.db_n && (alone || warp == 2)) p.db[c] = s * s_db;
+                }
+            }
+        }
+
+        for (int t = pair, n_tile = 0; t < num_items && ok; t += num_pairs, n_tile++) {
+            const Item it = item_of(p, t);
+            const Problem& q = *it.q;
             const int bn = it.tile.is_half ? BN / 2 : BN;
             const int m0 = it.tile.m_blk * BM + (int)rank * 128;
             const int n0 = it.tile.n_blk * BN + it.tile.half * (BN / 2);
             const int row = m0 + quarter * 32 + lane;
-            const bool valid = row < p.M;
-            float* bi = &sh->bias[0][0] + acc * acc_cols;
-            int label = -1;              // column of this launch, or out of its range
-            [[maybe_unused]] float row_max = 0.f, log2_sum = 0.f;
-            [[maybe_unused]] bool counts = false;
-            if constexpr (EPI != kSum) {
-                for (int c = et; c < bn; c += 32 * EPI_WARPS)
-                    bi[c] = p.bias && n0 + c < p.N ? p.bias[n0 + c] : 0.f;
-                if (valid) {
-                    if constexpr (EPI == kLse) {
-                        label = p.labels[row];
-                    } else {
-                        const int y = p.labels[row];
-                        row_max = p.stats[row];
-                        log2_sum = p.stats[(size_t)p.M + row] * LOG2E;
-                        // a row whose every entry is taken out (-inf) has no gradient
-                        counts = y != p.ignore && y >= 0 && y < p.vocab && row_max != -INFINITY;
-                        label = y - p.v0;
-                    }
-                }
-            }
-            [[maybe_unused]] float out_scale = 1.f;
-            if constexpr (EPI == kSum)
-                if (p.out) out_scale = p.count ? p.scale / fmaxf(*p.count, 1.f) : p.scale;
-            ok = tc::mbar_wait(tc::smem_u32(&sh->tmem_full[acc]), acc_phase, abort_flag, ERR_EPILOGUE);
-            ok = epilogue_all<32 * EPI_WARPS>(ok);
-            if (!ok) break;
-            tc::tc_fence_after();
-            const uint32_t taddr = tmem_base + acc * acc_cols + ((uint32_t)(quarter * 32) << 16);
+            const bool valid = row < q.M;
             const int c_first = colgrp * (bn / 2), c_end = c_first + bn / 2;
-            [[maybe_unused]] float top = -INFINITY, sum = 0.f;
+            uint32_t taddr;
 
-            auto emit = [&](uint32_t* r, int c) {      // 32 columns from tile column c
-                const int n = n0 + c;                  // output column
-                if constexpr (EPI == kSum) {
-                    if (!valid || n >= p.N) return;
-                    const size_t at = (size_t)row * p.N + n;
+            if constexpr (EPI == kSum) {
+                const uint32_t acc = take(taddr);
+                if (!ok) break;
+                const float out_scale = q.out ? (p.count ? p.scale / fmaxf(*p.count, 1.f) : p.scale) : 1.f;
+                auto emit = [&](uint32_t* r, int c) {
+                    const int n = n0 + c;
+                    if (!valid || n >= q.N) return;
+                    const size_t at = (size_t)row * q.N + n;
+                    if (q.add) {
 #pragma unroll
-                    for (int g = 0; g < 32; g += 8) {
-                        if (n + g >= p.N) break;       // N % 8 == 0: groups of eight are in or out together
-                        if (p.add) {
+                        for (int g = 0; g < 32; g += 8) {
+                            if (n + g >= q.N) break;       // N % 8 == 0: groups of eight are in or out together
                             float a[8];
-                            load8_f32(a, p.add + at + g);
+                            load8_f32(a, q.add + at + g);
 #pragma unroll
                             for (int j = 0; j < 8; j++) r[g + j] = __float_as_uint(__uint_as_float(r[g + j]) + a[j]);
                         }
                     }
-                    store_sum(p, r, at, n, it.split, out_scale);
-                } else {
-                    float f[32];
+                    store_sum(q, p.out_type, r, at, n, it.split, out_scale);
+                };
+                // a chunk is loaded from TMEM while the one before it is worked on
+                uint32_t ra[32], rb[32];
+                tc::tmem_ld_32x32(taddr + c_first, ra);
+#pragma unroll 1
+                for (int c = c_first; c < c_end; c += 64) {
+                    tc::tmem_ld_wait();
+                    tc::tmem_ld_32x32(taddr + c + 32, rb);
+                    emit(ra, c);
+                    tc::tmem_ld_wait();
+                    if (c + 64 < c_end) tc::tmem_ld_32x32(taddr + c + 64, ra);
+                    emit(rb, c + 32);
+                }
+                give_back(acc);
+            } else {
+                // Two bias buffers, by the tile's parity: the barrier in take() lies between the last reads of one
+                // and its next writes.
+                float* bi = sh->bias[n_tile & 1];
+                for (int c = et; c < bn; c += 32 * EPI_WARPS)
+                    bi[c] = p.bias && n0 + c < q.N ? p.bias[n0 + c] : 0.f;
+                int label = -1;              // column of this launch, or out of its range
+                if (valid) label = p.labels[row];
+                // W logits of this thread's row from tile column c: bias added, -inf past the vocabulary
+                auto logits = [&](float* f, int c, auto width) {
+                    constexpr int W = decltype(width)::value;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
+                    for (int j = 0; j < W; j += 8) {
                         float b8[8];
                         load8_f32(b8, bi + c + j);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) f[j + i] = __uint_as_float(r[j + i]) + b8[i];
+                        for (int i = 0; i < 8; i++) f[j + i] += b8[i];
                     }
-                    if (n + 32 > p.N) {                 // past the vocabulary: exp(-inf) = 0
+                    if (n0 + c + W > q.N) {
 #pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (n + j >= p.N) f[j] = -INFINITY;
+                        for (int j = 0; j < W; j++)
+                            if (n0 + c + j >= q.N) f[j] = -INFINITY;
                     }
-                    const int hit = label - n;          // the label's place in this chunk
-                    if constexpr (EPI == kLse) {
-                        if (hit >= 0 && hit < 32 && label < p.N) {
+                };
+                if constexpr (EPI == kLse) {
+                    float top = -INFINITY, sum = 0.f;
+                    // What the parts before the last one gave: 128 registers beside which 16 columns at a time
+                    // have room (168 registers a thread).
+                    constexpr int W = 16;
+                    float held[128 / W][W];
+                    const int parts = (it.kb1 + PART_KB - 1) / PART_KB;
+                    for (int part = 0; part + 1 < parts; part++) {
+                        const uint32_t acc = take(taddr);
+                        if (!ok) break;
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
+                        for (int i = 0; i < 128 / W; i++) {
+                            if (c_first + i * W >= c_end) continue;
+                            uint32_t r[W];
+                            tc::tmem_ld_32x16(taddr + c_first + i * W, r);
+                            tc::tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < W; j++)
+                                held[i][j] = part ? held[i][j] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
+                        }
+                        give_back(acc);
+                    }
+                    if (!ok) break;
+                    const uint32_t acc = take(taddr);
+                    if (!ok) break;
+#pragma unroll
+                    for (int i = 0; i < 128 / W; i++) {
+                        const int c = c_first + i * W;
+                        if (c >= c_end) continue;
+                        float f[W];
+                        tc::tmem_ld_32x16(taddr + c, (uint32_t*)f);
+                        tc::tmem_ld_wait();
+                        if (parts > 1) {
+#pragma unroll
+                            for (int j = 0; j < W; j++) f[j] += held[i][j];
+                        }
+                        logits(f, c, std::integral_constant<int, W>());
+                        const int hit = label - (n0 + c);          // the label's place in this chunk
+                        if (hit >= 0 && hit < W && label < q.N) {
+#pragma unroll
+                            for (int j = 0; j < W; j++)
                                 if (j == hit) p.label_logit[row] = f[j];
                         }
-                        float m = f[0];
+                        float m = top;
 #pragma unroll
-                        for (int j = 1; j < 32; j++) m = fmaxf(m, f[j]);
-                        m = fmaxf(m, top);
-                        // a row whose entries are all masked so far (-inf) has sum 0 relative to 0
+                        for (int j = 0; j < W; j++) m = fmaxf(m, f[j]);
+                        // a row whose entries are all taken out so far (-inf) has sum 0 relative to 0
                         const float ref = m == -INFINITY ? 0.f : m;
-                        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+                        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
+                        for (int j = 0; j < W; j += 2) {
                             s0 += ex2((f[j] - ref) * LOG2E);
                             s1 += ex2((f[j + 1] - ref) * LOG2E);
-                            s2 += ex2((f[j + 2] - ref) * LOG2E);
-                            s3 += ex2((f[j + 3] - ref) * LOG2E);
                         }
-                        sum = sum * ex2((top - ref) * LOG2E) + ((s0 + s1) + (s2 + s3));
+                        sum = sum * ex2((top - ref) * LOG2E) + (s0 + s1);
                         top = m;
-                    } else {
+                    }
+                    give_back(acc);
+                    // the joined maximum and sum of this warp's columns, for each of its rows (kLse tiles are never
+                    // cut in two, so a 256-column block has these two entries)
+                    if (valid) p.partial[(size_t)(it.tile.n_blk * 2 + colgrp) * q.M + row] = make_float2(top, sum);
+                } else {
+                    float row_max = 0.f, log2_sum = 0.f;
+                    bool counts = false;
+                    if (valid) {
+                        row_max = p.stats[row];
+                        log2_sum = p.stats[(size_t)q.M + row] * LOG2E;
+                        // a row whose every entry is taken out (-inf) has no gradient
+                        counts = label != p.ignore && label >= 0 && label < p.vocab && row_max != -INFINITY;
+                        label -= p.v0;
+                    }
+                    const uint32_t acc = take(taddr);
+                    if (!ok) break;
+                    auto emit = [&](const uint32_t* r, int c) {
+                        const int n = n0 + c;
+                        float f[32];
+#pragma unroll
+                        for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
+                        logits(f, c, std::integral_constant<int, 32>());
 #pragma unroll
                         for (int j = 0; j < 32; j++) f[j] = ex2(fmaf(f[j] - row_max, LOG2E, -log2_sum));
+                        const int hit = label - n;
                         if (hit >= 0 && hit < 32) {
 #pragma unroll
                             for (int j = 0; j < 32; j++)
@@ -404,33 +534,24 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                                     f[j] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, h);
                                 }
                             }
-                            if (n + lane < p.ldp && m0 + quarter * 32 < p.M)
+                            if (n + lane < p.ldp && m0 + quarter * 32 < q.M)
                                 p.col_partial[(size_t)((m0 >> 5) + quarter) * p.ldp + n + lane] = f[0];
                         }
-                    }
-                }
-            };
-            // a chunk is loaded from TMEM while the one before it is worked on
-            uint32_t ra[32], rb[32];
-            tc::tmem_ld_32x32(taddr + c_first, ra);
+                    };
+                    uint32_t ra[32], rb[32];
+                    tc::tmem_ld_32x32(taddr + c_first, ra);
 #pragma unroll 1
-            for (int c = c_first; c < c_end; c += 64) {
-                tc::tmem_ld_wait();
-                if (c + 32 < c_end) tc::tmem_ld_32x32(taddr + c + 32, rb);
-                emit(ra, c);
-                if (c + 32 < c_end) {
-                    tc::tmem_ld_wait();
-                    if (c + 64 < c_end) tc::tmem_ld_32x32(taddr + c + 64, ra);
-                    emit(rb, c + 32);
+                    for (int c = c_first; c < c_end; c += 64) {
+                        tc::tmem_ld_wait();
+                        tc::tmem_ld_32x32(taddr + c + 32, rb);
+                        emit(ra, c);
+                        tc::tmem_ld_wait();
+                        if (c + 64 < c_end) tc::tmem_ld_32x32(taddr + c + 64, ra);
+                        emit(rb, c + 32);
+                    }
+                    give_back(acc);
                 }
             }
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive_remote(tc::mapa(tc::smem_u32(&sh->tmem_empty[acc]), 0));
-            // the joined maximum and sum of this warp's columns, for each of its rows (kLse tiles are never
-            // cut in two, so a 256-column block has these two entries)
-            if constexpr (EPI == kLse)
-                if (valid) p.partial[(size_t)(it.tile.n_blk * 2 + colgrp) * p.M + row] = make_float2(top, sum);
         }
     }
 
@@ -447,8 +568,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 }
 
 // ---------------------------------------------------------------- joining what the tiles left
-// Row statistics, row loss and the label checks: 32 rows per block, one per lane, the partial maxima and sums
-// dealt out to the warps.  The sum of the block's row losses and its count of rows go to block_sum.
+// Row statistics, row loss and the label checks, one row per lane.
 constexpr int JOIN_WARPS = 32;
 
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
@@ -458,62 +578,81 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = top;
 }
 
+// loss[0] = sum of the row losses (over their count for the mean; 0 when no row counts), loss[1] = count
+__device__ __forceinline__ void put_loss(float* loss, double sum, double count, int mean) {
+    loss[0] = (float)(mean ? sum / (count > 1.0 ? count : 1.0) : sum);
+    loss[1] = (float)count;
+}
+
+// WAYS warps share 32 rows; a block takes 32 / WAYS groups of rows.  With one block the loss is complete.
+template <int WAYS>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
-join_lse_kernel(float* __restrict__ stats, float* __restrict__ row_loss, float2* __restrict__ block_sum,
-                const float2* __restrict__ partial, const float* __restrict__ label_logit,
-                const int32_t* __restrict__ labels, int M, int slots, int vocab, int ignore, int* __restrict__ status) {
-    __shared__ float2 part[JOIN_WARPS][32];
+join_rows_kernel(float* __restrict__ loss_out, float* __restrict__ stats, float* __restrict__ row_loss,
+                 double2* __restrict__ block_sum, const float2* __restrict__ partial,
+                 const float* __restrict__ label_logit, const int32_t* __restrict__ labels, int M, int slots, int vocab,
+                 int ignore, int mean, int* __restrict__ status) {
+    __shared__ float2 part[WAYS > 1 ? JOIN_WARPS : 1][32];
+    __shared__ double sums[JOIN_WARPS], counts[JOIN_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x * 32 + lane;
+    const int row = (blockIdx.x * (JOIN_WARPS / WAYS) + warp / WAYS) * 32 + lane;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     float m = -INFINITY, s = 0.f;
     if (row < M) {
-        int i = warp;
-        for (; i + 3 * JOIN_WARPS < slots; i += 4 * JOIN_WARPS) {
+        int i = warp % WAYS;
+        for (; i + 3 * WAYS < slots; i += 4 * WAYS) {
             float2 q[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) q[k] = partial[(size_t)(i + k * JOIN_WARPS) * M + row];
+            for (int k = 0; k < 4; k++) q[k] = partial[(size_t)(i + k * WAYS) * M + row];
 #pragma unroll
             for (int k = 0; k < 4; k++) join(m, s, q[k].x, q[k].y);
         }
-        for (; i < slots; i += JOIN_WARPS) {
+        for (; i < slots; i += WAYS) {
             const float2 q = partial[(size_t)i * M + row];
             join(m, s, q.x, q.y);
         }
     }
-    part[warp][lane] = make_float2(m, s);
-    __syncthreads();
-    if (warp != 0) return;
-    for (int w = 1; w < JOIN_WARPS; w++) join(m, s, part[w][lane].x, part[w][lane].y);
-    float loss = 0.f, n = 0.f;
-    if (row < M) {
+    if constexpr (WAYS > 1) {
+        part[warp][lane] = make_float2(m, s);
+        __syncthreads();
+        if (warp % WAYS == 0)
+            for (int w = 1; w < WAYS; w++) join(m, s, part[warp + w][lane].x, part[warp + w][lane].y);
+    }
+    double loss = 0.0, n = 0.0;
+    if (warp % WAYS == 0 && row < M) {
         // maximum and logarithm are kept apart: their sum would lose the logarithm where the logits are large
         const float log_sum = m == -INFINITY ? 0.f : logf(s);
         const int y = labels[row];
+        float mine = 0.f;
         if (y != ignore) {
             if (y >= 0 && y < vocab) {
-                loss = m == -INFINITY ? INFINITY : (m - label_logit[row]) + log_sum;
-                n = 1.f;
+                mine = m == -INFINITY ? INFINITY : (m - label_logit[row]) + log_sum;
+                n = 1.0;
             } else if (status) {
                 atomicCAS(status, 0, (int)ERR_LABEL);
             }
         }
+        loss = mine;
         stats[row] = m;
         stats[(size_t)M + row] = log_sum;
-        if (row_loss) row_loss[row] = loss;
+        if (row_loss) row_loss[row] = mine;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         loss += __shfl_xor_sync(0xFFFFFFFFu, loss, o);
         n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
     }
-    if (lane == 0) block_sum[blockIdx.x] = make_float2(loss, n);
+    if (lane == 0) { sums[warp] = loss; counts[warp] = n; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < JOIN_WARPS; w++) { loss += sums[w]; n += counts[w]; }
+        if (gridDim.x == 1) put_loss(loss_out, loss, n, mean);
+        else block_sum[blockIdx.x] = make_double2(loss, n);
+    }
 }
 
-// loss[0] = sum of the row losses (over their count for the mean; 0 when no row counts), loss[1] = count
 __global__ void __launch_bounds__(256)
-loss_kernel(float* __restrict__ loss, const float2* __restrict__ block_sum, int blocks, int mean) {
-    __shared__ double sum[8], num[8];
+loss_kernel(float* __restrict__ loss_out, const double2* __restrict__ block_sum, int blocks, int mean) {
+    __shared__ double sums[8], counts[8];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     double s = 0.0, n = 0.0;
     for (int i = threadIdx.x; i < blocks; i += 256) {
@@ -525,12 +664,11 @@ loss_kernel(float* __restrict__ loss, const float2* __restrict__ block_sum, int 
         s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
         n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
     }
-    if ((threadIdx.x & 31) == 0) { sum[threadIdx.x >> 5] = s; num[threadIdx.x >> 5] = n; }
+    if ((threadIdx.x & 31) == 0) { sums[threadIdx.x >> 5] = s; counts[threadIdx.x >> 5] = n; }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; w++) { s += sum[w]; n += num[w]; }
-        loss[0] = (float)(mean ? s / (n > 1.0 ? n : 1.0) : s);
-        loss[1] = (float)n;
+        for (int w = 1; w < 8; w++) { s += sums[w]; n += counts[w]; }
+        put_loss(loss_out, s, n, mean);
     }
 }
 
@@ -599,48 +737,57 @@ nvq_status launch_after(void (*kernel)(KArgs...), size_t grid, int threads, int 
     return NVQ_OK;
 }
 
-template <int EPI, bool A_MN, bool B_MN>
-nvq_status launch_gemm(CeParams& p, const CUtensorMap& a, const CUtensorMap& b, int device, cudaStream_t st) {
+template <int EPI>
+nvq_status launch_gemm(CeParams& p, const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
+                       const CUtensorMap& b1, int device, cudaStream_t st) {
     static std::atomic<bool> attr_set[64];   // per device; setting the attribute twice is harmless
     if (!attr_set[device]) {
-        NVQ_CUDA(cudaFuncSetAttribute(ce_gemm_kernel<EPI, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      SMEM_BYTES));
+        NVQ_CUDA(cudaFuncSetAttribute(ce_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
         attr_set[device] = true;
     }
     nvq_status s = nvq_status_word(device, &p.status);
     if (s != NVQ_OK) return s;
-    p.m_blocks = (p.M + BM - 1) / BM;
-    p.n_blocks = (p.N + BN - 1) / BN;
-    p.group_m = 8;
-    const int tiles = p.m_blocks * p.n_blocks, pairs = nvq_sm_count(device) / 2;
-    p.num_big = p.num_items = tiles * p.splits;
-    if (EPI != kLse && p.splits == 1 && p.N > BN / 2) {
-        // a partial last wave that would occupy at most half of the pairs is cut into half-width tiles
-        const int rem = tiles % pairs;
-        const int cut = tiles > pairs && rem > 0 && 2 * rem <= pairs ? rem : 0;
-        p.num_big = tiles - cut;
-        p.num_items = p.num_big + 2 * cut;
+    const int pairs = nvq_sm_count(device) / 2;
+    for (Problem& q : p.q) {
+        q.m_blocks = (q.M + BM - 1) / BM;
+        q.n_blocks = (q.N + BN - 1) / BN;
+        q.group_m = 8;
+        q.num_big = q.num_items = q.m_blocks * q.n_blocks * q.splits;
     }
-    const int used = p.num_items < pairs ? p.num_items : pairs;
-    return launch_after(ce_gemm_kernel<EPI, A_MN, B_MN>, 2 * (size_t)used, THREADS, SMEM_BYTES, st, a, b, p);
+    // a partial last wave that would occupy at most half of the pairs is cut into half-width tiles
+    Problem& tail = p.q[p.q[1].num_items ? 1 : 0];
+    const int total = p.q[0].num_items + p.q[1].num_items, rem = total % pairs;
+    if (EPI != kLse && tail.splits == 1 && tail.N > BN / 2 && total > pairs && 2 * rem <= pairs && rem <= tail.num_items) {
+        tail.num_big -= rem;
+        tail.num_items += rem;
+    }
+    const int items = p.q[0].num_items + p.q[1].num_items;
+    const int used = items < pairs ? items : pairs;
+    return launch_after(ce_gemm_kernel<EPI>, 2 * (size_t)used, THREADS, SMEM_BYTES, st, a0, b0, a1, b1, p);
 }
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
-// A contraction with fewer output tiles than half the CTA pairs is cut along its length, four k-blocks
-// at least in a part, so that every pair has one.
-struct Split { int splits, kb_per; };
-Split split_of(size_t M, size_t N, size_t K, int pairs) {
-    const size_t tiles = (M + BM - 1) / BM * ((N + BN - 1) / BN);
-    const int num_kb = (int)((K + BK - 1) / BK);
-    int want = tiles * 2 > (size_t)pairs ? 1 : (int)(pairs / tiles);
-    if (want > num_kb / 4) want = num_kb / 4;
-    if (want < 1) want = 1;
-    Split s;
-    s.kb_per = (num_kb + want - 1) / want;
-    s.splits = (num_kb + s.kb_per - 1) / s.kb_per;
-    return s;
+constexpr int kPairs = 74;      // what the splits are made for: workspace sizes are asked for without a device
+
+// The contractions of one launch as tiles and their length in k-blocks; splits[i] > 1: one item of a tile would take longer
+// than an even share of all work, and the tile is cut into parts of about that share, eight k-blocks at least.
+struct Shape { size_t M, N, K; };
+struct Cut { int splits, kb_per; };
+void cut_long(const Shape* q, Cut* cut, int n) {
+    size_t total = 0;
+    for (int i = 0; i < n; i++) total += (q[i].M + BM - 1) / BM * ((q[i].N + BN - 1) / BN) * ((q[i].K + BK - 1) / BK);
+    size_t share = (total + kPairs - 1) / kPairs;
+    if (share < 8) share = 8;
+    for (int i = 0; i < n; i++) {
+        const size_t kb = (q[i].K + BK - 1) / BK;
+        size_t parts = (kb + share - 1) / share;
+        if (parts < 1) parts = 1;
+        cut[i].kb_per = (int)((kb + parts - 1) / parts);
+        cut[i].splits = (int)((kb + cut[i].kb_per - 1) / cut[i].kb_per);
+    }
 }
+size_t part_bytes(const Shape& q, const Cut& c) { return c.splits > 1 ? align256(c.splits * q.M * q.N * 4) : 0; }
 
 // Vocabulary entries per piece of the backward pass: 64 Mi values of g, 8192 entries at least, so that adding a
 // piece to the fp32 dX costs little beside its contractions.
@@ -657,53 +804,52 @@ FwdSpace fwd_space(size_t M, size_t V) {
     FwdSpace s;
     s.partial = align256((V + BN - 1) / BN * 2 * M * sizeof(float2));
     s.logit = align256(M * 4);
-    s.block = align256((M + 31) / 32 * sizeof(float2));
+    s.block = align256((M + 31) / 32 * sizeof(double2));
     s.total = s.partial + s.logit + s.block;
     return s;
 }
-struct BwdSpace { size_t prob, cols, sum, parts, total; };
-BwdSpace bwd_space(size_t M, size_t V, size_t K, int pairs) {
+
+// Parts of the split contractions of one piece, whichever of dX and dW are wanted
+size_t parts_space(size_t M, size_t nv, size_t K) {
+    const Shape q[2] = {{M, K, nv}, {nv, K, M}};
+    Cut c[2];
+    cut_long(q, c, 2);
+    size_t most = part_bytes(q[0], c[0]) + part_bytes(q[1], c[1]);
+    for (int i = 0; i < 2; i++) {
+        cut_long(q + i, c + i, 1);
+        const size_t one = part_bytes(q[i], c[i]);
+        if (one > most) most = one;
+    }
+    return most;
+}
+struct BwdSpace { size_t prob, cols, sum, total; };
+BwdSpace bwd_space(size_t M, size_t V, size_t K) {
     BwdSpace s;
     const size_t piece = piece_of(M, V), nv = piece < V ? piece : V, ld = (nv + 15) / 16 * 16;
     s.prob = align256(M * ld * 2);
     s.cols = align256((M + 31) / 32 * ld * 4);
     s.sum = piece < V ? align256(M * K * 4) : 0;
-    const Split x = split_of(M, K, nv, pairs), w = split_of(nv, K, M, pairs);
-    const size_t px = x.splits > 1 ? x.splits * M * K * 4 : 0, pw = w.splits > 1 ? w.splits * nv * K * 4 : 0;
-    // the last piece may be shorter, and its split another one: its parts are never more than a wave of tiles
-    const size_t wave = (size_t)pairs * BM * BN * 4;
-    size_t parts = px > pw ? px : pw;
-    if (piece < V && parts < wave) parts = wave;
-    s.parts = align256(parts);
-    s.total = s.prob + s.cols + s.sum + s.parts;
+    size_t parts = parts_space(M, nv, K);
+    if (V % piece && piece < V) {       // the last, shorter piece
+        const size_t last = parts_space(M, V % piece, K);
+        if (last > parts) parts = last;
+    }
+    s.total = s.prob + s.cols + s.sum + parts;
     return s;
 }
 
-constexpr int kDefaultPairs = 74;      // sizes are asked for without a device
-
-template <bool A_MN, bool B_MN>
-nvq_status contract(CeParams& p, const CUtensorMap& a, const CUtensorMap& b, float* parts, int device, cudaStream_t st) {
-    const Split sp = split_of(p.M, p.N, p.K, kDefaultPairs);
-    p.splits = sp.splits;
-    p.kb_per = sp.kb_per;
-    if (sp.splits == 1) return launch_gemm<kSum, A_MN, B_MN>(p, a, b, device, st);
-    CeParams q = p;
-    q.out = nullptr;
-    q.add = nullptr;
-    q.sum = parts;
-    nvq_status s = launch_gemm<kSum, A_MN, B_MN>(q, a, b, device, st);
-    if (s != NVQ_OK) return s;
-    const size_t n = (size_t)p.M * p.N, grid = (n / 4 + 255) / 256;
-    if (p.out == nullptr)
-        return launch_after(join_splits_kernel<NVQ_F32>, grid, 256, 0, st, (void*)p.sum, parts, sp.splits, p.add, n, 1.f,
+nvq_status join_parts(const Problem& q, const CeParams& p, const float* parts, cudaStream_t st) {
+    const size_t n = (size_t)q.M * q.N, grid = (n / 4 + 255) / 256;
+    if (q.out == nullptr)
+        return launch_after(join_splits_kernel<NVQ_F32>, grid, 256, 0, st, (void*)q.sum, parts, q.splits, q.add, n, 1.f,
                             nullptr);
     if (p.out_type == NVQ_F32)
-        return launch_after(join_splits_kernel<NVQ_F32>, grid, 256, 0, st, p.out, parts, sp.splits, p.add, n, p.scale,
+        return launch_after(join_splits_kernel<NVQ_F32>, grid, 256, 0, st, q.out, parts, q.splits, q.add, n, p.scale,
                             p.count);
     if (p.out_type == NVQ_F16)
-        return launch_after(join_splits_kernel<NVQ_F16>, grid, 256, 0, st, p.out, parts, sp.splits, p.add, n, p.scale,
+        return launch_after(join_splits_kernel<NVQ_F16>, grid, 256, 0, st, q.out, parts, q.splits, q.add, n, p.scale,
                             p.count);
-    return launch_after(join_splits_kernel<NVQ_BF16>, grid, 256, 0, st, p.out, parts, sp.splits, p.add, n, p.scale,
+    return launch_after(join_splits_kernel<NVQ_BF16>, grid, 256, 0, st, q.out, parts, q.splits, q.add, n, p.scale,
                         p.count);
 }
 
@@ -732,7 +878,7 @@ extern "C" nvq_status nvq_linear_ce_workspace_bytes(size_t M, size_t V, size_t K
     if (M == 0) return NVQ_OK;
     *bytes = fwd_space(M, V).total;
     if (backward) {
-        const size_t b = bwd_space(M, V, K, kDefaultPairs).total;
+        const size_t b = bwd_space(M, V, K).total;
         if (b > *bytes) *bytes = b;
     }
     return NVQ_OK;
@@ -765,25 +911,30 @@ extern "C" nvq_status nvq_linear_ce_fwd(float* d_loss_count, float* d_row_loss, 
     char* ws = (char*)d_workspace;
     float2* partial = (float2*)ws;
     float* logit = (float*)(ws + sp.partial);
-    float2* block_sum = (float2*)(ws + sp.partial + sp.logit);
+    double2* block_sum = (double2*)(ws + sp.partial + sp.logit);
     CeParams p = {};
-    p.M = (int)M;
-    p.N = (int)V;
-    p.K = (int)K;
-    p.splits = 1;
+    p.q[0].M = (int)M;
+    p.q[0].N = (int)V;
+    p.q[0].K = (int)K;
+    p.q[0].splits = 1;
     p.f16 = dtype == NVQ_F16;
     p.bias = d_bias;
     p.labels = d_labels;
     p.partial = partial;
     p.label_logit = logit;
-    s = launch_gemm<kLse, false, false>(p, a, b, device, st);
+    s = launch_gemm<kLse>(p, a, b, a, b, device, st);
     if (s != NVQ_OK) return s;
-    const int blocks = (int)((M + 31) / 32), slots = 2 * p.n_blocks;
-    s = launch_after(join_lse_kernel, blocks, JOIN_WARPS * 32, 0, st, d_row_stats, d_row_loss, block_sum, partial, logit,
-                     d_labels, (int)M, slots, (int)V, ignore_index, p.status);
-    if (s != NVQ_OK) return s;
-    return launch_after(loss_kernel, 1, 256, 0, st, d_loss_count, block_sum, blocks,
-                        (int)(reduction == NVQ_REDUCE_MEAN));
+    // up to eight partial sums a row: a warp adds up 32 rows by itself; more: the whole block does
+    const int slots = 2 * p.q[0].n_blocks, mean = reduction == NVQ_REDUCE_MEAN;
+    const int rows = slots <= 8 ? 32 * JOIN_WARPS : 32, blocks = (int)((M + rows - 1) / rows);
+    s = slots <= 8 ? launch_after(join_rows_kernel<1>, blocks, JOIN_WARPS * 32, 0, st, d_loss_count, d_row_stats,
+                                  d_row_loss, block_sum, partial, logit, d_labels, (int)M, slots, (int)V, ignore_index,
+                                  mean, p.status)
+                   : launch_after(join_rows_kernel<JOIN_WARPS>, blocks, JOIN_WARPS * 32, 0, st, d_loss_count,
+                                  d_row_stats, d_row_loss, block_sum, partial, logit, d_labels, (int)M, slots, (int)V,
+                                  ignore_index, mean, p.status);
+    if (s != NVQ_OK || blocks == 1) return s;
+    return launch_after(loss_kernel, 1, 256, 0, st, d_loss_count, block_sum, blocks, mean);
 }
 
 extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_dtype, float* d_db, const void* d_x,
@@ -801,7 +952,7 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
                 "nvq_linear_ce_bwd: needs the row statistics, loss and count that nvq_linear_ce_fwd left");
     const size_t size = grad_dtype == NVQ_F32 ? 4 : 2;
     BwdSpace sp = {};
-    if (M) sp = bwd_space(M, V, K, kDefaultPairs);
+    if (M) sp = bwd_space(M, V, K);
     NVQ_REQUIRE(M == 0 || (d_workspace && workspace_bytes >= sp.total && nvq_aligned(d_workspace, 256)),
                 "nvq_linear_ce_bwd: workspace of %zu bytes (256-byte aligned) required", sp.total);
     s = nvq_use_device(device);
@@ -817,9 +968,8 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
     uint16_t* prob = (uint16_t*)ws;
     float* cols = (float*)(ws + sp.prob);
     float* sum = (float*)(ws + sp.prob + sp.cols);
-    float* parts = (float*)(ws + sp.prob + sp.cols + sp.sum);
+    char* parts = ws + sp.prob + sp.cols + sp.sum;
     const float* count = reduction == NVQ_REDUCE_MEAN ? d_loss_count + 1 : nullptr;
-    const float gain = dtype == NVQ_F16 ? F16_GAIN : 1.f;
     const size_t piece = piece_of(M, V);
     CUtensorMap x_k, x_mn;      // X with the contraction along its rows, and across them
     s = nvq_make_tmap_2d(&x_k, d_x, M, K, 128, BK, 2, 1);
@@ -828,6 +978,7 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
     if (s != NVQ_OK) return s;
     for (size_t v0 = 0; v0 < V; v0 += piece) {
         const size_t nv = V - v0 < piece ? V - v0 : piece, ld = (nv + 15) / 16 * 16;
+        const bool last = v0 + nv == V;
         const uint16_t* w = (const uint16_t*)d_w + v0 * K;
         CUtensorMap w_k, w_mn, g_k, g_mn;
         if ((s = nvq_make_tmap_2d(&w_k, w, nv, K, 64, BK, 2, 1)) != NVQ_OK) return s;
@@ -835,10 +986,10 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
         if ((s = nvq_make_tmap_2d(&g_k, prob, M, ld, 128, BK, 2, 1)) != NVQ_OK) return s;
         if ((s = nvq_make_tmap_2d(&g_mn, prob, M, ld, BK, 64, 2, 1)) != NVQ_OK) return s;
         CeParams p = {};
-        p.M = (int)M;
-        p.N = (int)nv;
-        p.K = (int)K;
-        p.splits = 1;
+        p.q[0].M = (int)M;
+        p.q[0].N = (int)nv;
+        p.q[0].K = (int)K;
+        p.q[0].splits = 1;
         p.f16 = dtype == NVQ_F16;
         p.bias = d_bias ? d_bias + v0 : nullptr;
         p.labels = d_labels;
@@ -849,42 +1000,70 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
         p.prob = prob;
         p.ldp = (int)ld;
         p.col_partial = d_db ? cols : nullptr;
-        s = launch_gemm<kProb, false, false>(p, x_k, w_k, device, st);
+        s = launch_gemm<kProb>(p, x_k, w_k, x_k, w_k, device, st);
         if (s != NVQ_OK) return s;
-        if (d_db) {
-            s = launch_after(bias_grad_kernel, (nv + 31) / 32, 256, 0, st, d_db + v0, cols, (int)((M + 31) / 32),
-                             (int)ld, (int)nv, grad_scale, count);
-            if (s != NVQ_OK) return s;
+
+        // dX and dW of the piece in one launch, and db beside them
+        CeParams u = {};
+        u.f16 = p.f16;
+        u.out_type = grad_dtype;
+        u.scale = grad_scale / (p.f16 ? F16_GAIN : 1.f);
+        u.count = count;
+        u.col_partial = cols;
+        u.ldp = (int)ld;
+        u.db = d_db ? d_db + v0 : nullptr;
+        u.db_n = (int)nv;
+        u.groups = (int)((M + 31) / 32);
+        u.db_scale = grad_scale;
+        Problem dx = {}, dw = {};
+        dx.M = (int)M;
+        dx.N = dw.N = (int)K;
+        dx.K = dw.M = (int)nv;
+        dw.K = (int)M;
+        dw.a_mn = 1;
+        dx.add = v0 ? sum : nullptr;
+        dx.sum = last ? nullptr : sum;
+        dx.out = last ? d_dx : nullptr;
+        dx.vec32 = K * size % 32 == 0 && nvq_aligned(d_dx, 32);
+        dw.out = d_dw ? (char*)d_dw + v0 * K * size : nullptr;
+        dw.vec32 = K * size % 32 == 0 && nvq_aligned(d_dw, 32);
+        Shape shape[2];
+        Cut cut[2];
+        Problem* wanted[2];
+        int n = 0;
+        if (d_dx) { shape[n] = {M, K, nv}; wanted[n++] = &dx; }
+        if (d_dw) { shape[n] = {nv, K, M}; wanted[n++] = &dw; }
+        cut_long(shape, cut, n);
+        char* at = parts;
+        Problem whole[2];              // as wanted, for joining the parts
+        for (int i = 0; i < n; i++) {
+            Problem& q = *wanted[i];
+            q.splits = cut[i].splits;
+            q.kb_per = cut[i].kb_per;
+            whole[i] = q;
+            if (q.splits > 1) {
+                q.add = nullptr;
+                q.out = nullptr;
+                q.sum = (float*)at;
+                at += part_bytes(shape[i], cut[i]);
+            }
         }
-        if (d_dx) {
-            const bool last = v0 + nv == V;
-            CeParams q = {};
-            q.M = (int)M;
-            q.N = (int)K;
-            q.K = (int)nv;
-            q.f16 = p.f16;
-            q.add = v0 ? sum : nullptr;
-            q.sum = last ? nullptr : sum;
-            q.out = last ? d_dx : nullptr;
-            q.out_type = grad_dtype;
-            q.vec32 = K * size % 32 == 0 && nvq_aligned(d_dx, 32);
-            q.scale = grad_scale / gain;
-            q.count = count;
-            s = contract<false, true>(q, g_k, w_mn, parts, device, st);
-            if (s != NVQ_OK) return s;
+        // the longer items first
+        const bool swap = n == 2 && cut[1].kb_per > cut[0].kb_per;
+        if (n > 0) u.q[swap ? 1 : 0] = *wanted[0];
+        if (n > 1) u.q[swap ? 0 : 1] = *wanted[1];
+        const bool first_dw = n > 0 && wanted[swap ? 1 : 0] == &dw;
+        if (n == 0) {
+            s = launch_after(bias_grad_kernel, (nv + 31) / 32, 256, 0, st, u.db, cols, u.groups, u.ldp, u.db_n, grad_scale,
+                             count);
+        } else {
+            s = first_dw ? launch_gemm<kSum>(u, g_mn, x_mn, g_k, w_mn, device, st)
+                         : launch_gemm<kSum>(u, g_k, w_mn, g_mn, x_mn, device, st);
         }
-        if (d_dw) {
-            CeParams q = {};
-            q.M = (int)nv;
-            q.N = (int)K;
-            q.K = (int)M;
-            q.f16 = p.f16;
-            q.out = (char*)d_dw + v0 * K * size;
-            q.out_type = grad_dtype;
-            q.vec32 = K * size % 32 == 0 && nvq_aligned(d_dw, 32);
-            q.scale = grad_scale / gain;
-            q.count = count;
-            s = contract<true, true>(q, g_mn, x_mn, parts, device, st);
+        if (s != NVQ_OK) return s;
+        for (int i = 0; i < n; i++) {
+            if (cut[i].splits == 1) continue;
+            s = join_parts(whole[i], u, wanted[i]->sum, st);
             if (s != NVQ_OK) return s;
         }
     }
