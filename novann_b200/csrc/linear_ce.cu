@@ -86,6 +86,38 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Keeps what follows a wait for TMEM loads behind it: the loaded registers are touched here.
+template <int N>
+__device__ __forceinline__ void pin(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
+}
+
 // Shared-memory descriptor of a tile whose rows run along the contraction and hold 64 elements of the
 // other dimension (128 bytes, 128-byte swizzle): groups of 8 rows are 1024 bytes apart, the next 64
 // elements of the other dimension 64 rows (8192 bytes) further on.
@@ -400,156 +432,172 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                 for (int c = et; c < bn; c += 32 * EPI_WARPS)
                     bi[c] = p.bias && n0 + c < q.N ? p.bias[n0 + c] : 0.f;
                 int label = -1;              // column of this launch, or out of its range
-                if (valid) label = p.labels[row];
-                // W logits of this thread's row from tile column c: bias added, -inf past the vocabulary
-                auto logits = [&](float* f, int c, auto width) {
-                    constexpr int W = decltype(width)::value;
-#pragma unroll
-                    for (int j = 0; j < W; j += 8) {
-                        float b8[8];
-                        load8_f32(b8, bi + c + j);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) f[j + i] += b8[i];
-                    }
-                    if (n0 + c + W > q.N) {
-#pragma unroll
-                        for (int j = 0; j < W; j++)
-                            if (n0 + c + j >= q.N) f[j] = -INFINITY;
-                    }
-                };
-                if constexpr (EPI == kLse) {
-                    float top = -INFINITY, sum = 0.f;
-                    // What the parts before the last one gave: 128 registers beside which 16 columns at a time
-                    // have room (168 registers a thread).
-                    constexpr int W = 16;
-                    float held[128 / W][W];
-                    const int parts = (it.kb1 + PART_KB - 1) / PART_KB;
-                    for (int part = 0; part + 1 < parts; part++) {
-                        const uint32_t acc = take(taddr);
-                        if (!ok) break;
-#pragma unroll
-                        for (int i = 0; i < 128 / W; i++) {
-                            if (c_first + i * W >= c_end) continue;
-                            uint32_t r[W];
-                            tc::tmem_ld_32x16(taddr + c_first + i * W, r);
-                            tc::tmem_ld_wait();
-#pragma unroll
-                            for (int j = 0; j < W; j++)
-                                held[i][j] = part ? held[i][j] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
-                        }
-                        give_back(acc);
-                    }
-                    if (!ok) break;
-                    const uint32_t acc = take(taddr);
-                    if (!ok) break;
-#pragma unroll
-                    for (int i = 0; i < 128 / W; i++) {
-                        const int c = c_first + i * W;
-                        if (c >= c_end) continue;
-                        float f[W];
-                        tc::tmem_ld_32x16(taddr + c, (uint32_t*)f);
-                        tc::tmem_ld_wait();
-                        if (parts > 1) {
-#pragma unroll
-                            for (int j = 0; j < W; j++) f[j] += held[i][j];
-                        }
-                        logits(f, c, std::integral_constant<int, W>());
-                        const int hit = label - (n0 + c);          // the label's place in this chunk
-                        if (hit >= 0 && hit < W && label < q.N) {
-#pragma unroll
-                            for (int j = 0; j < W; j++)
-                                if (j == hit) p.label_logit[row] = f[j];
-                        }
-                        float m = top;
-#pragma unroll
-                        for (int j = 0; j < W; j++) m = fmaxf(m, f[j]);
-                        // a row whose entries are all taken out so far (-inf) has sum 0 relative to 0
-                        const float ref = m == -INFINITY ? 0.f : m;
-                        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-                        for (int j = 0; j < W; j += 2) {
-                            s0 += ex2((f[j] - ref) * LOG2E);
-                            s1 += ex2((f[j + 1] - ref) * LOG2E);
-                        }
-                        sum = sum * ex2((top - ref) * LOG2E) + (s0 + s1);
-                        top = m;
-                    }
-                    give_back(acc);
-                    // the joined maximum and sum of this warp's columns, for each of its rows (kLse tiles are never
-                    // cut in two, so a 256-column block has these two entries)
-                    if (valid) p.partial[(size_t)(it.tile.n_blk * 2 + colgrp) * q.M + row] = make_float2(top, sum);
-                } else {
-                    float row_max = 0.f, log2_sum = 0.f;
-                    bool counts = false;
-                    if (valid) {
+                [[maybe_unused]] float row_max = 0.f, log2_sum = 0.f;
+                [[maybe_unused]] bool counts = false;
+                if (valid) {
+                    label = p.labels[row];
+                    if constexpr (EPI == kProb) {
                         row_max = p.stats[row];
                         log2_sum = p.stats[(size_t)q.M + row] * LOG2E;
                         // a row whose every entry is taken out (-inf) has no gradient
                         counts = label != p.ignore && label >= 0 && label < p.vocab && row_max != -INFINITY;
                         label -= p.v0;
                     }
-                    const uint32_t acc = take(taddr);
-                    if (!ok) break;
-                    auto emit = [&](const uint32_t* r, int c) {
-                        const int n = n0 + c;
-                        float f[32];
+                }
+                const int width = bn / 2;                 // columns of this warp: 128, or 64 of a half-width tile
+                const int n_first = n0 + c_first;
+                float v[128];
+                // All columns of this warp lie in registers before anything is done with them: the loads overlap, the
+                // accumulator goes back at once, and maximum and sum run over 128 independent values.
+                uint32_t acc = take(taddr);
+                if (!ok) break;
 #pragma unroll
-                        for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
-                        logits(f, c, std::integral_constant<int, 32>());
+                for (int i = 0; i < 4; i++)
+                    if (i * 32 < width) tc::tmem_ld_32x32(taddr + c_first + i * 32, (uint32_t*)v + i * 32);
+                tc::tmem_ld_wait();
+                pin(v);
+                give_back(acc);
+                if constexpr (EPI == kLse) {
+                    for (int k0 = PART_KB; k0 < it.kb1; k0 += PART_KB) {
+                        acc = take(taddr);
+                        if (!ok) break;
 #pragma unroll
-                        for (int j = 0; j < 32; j++) f[j] = ex2(fmaf(f[j] - row_max, LOG2E, -log2_sum));
-                        const int hit = label - n;
-                        if (hit >= 0 && hit < 32) {
+                        for (int i = 0; i < 8; i++) {
+                            if (i * 16 >= width) continue;
+                            float r[16];
+                            tc::tmem_ld_32x16(taddr + c_first + i * 16, (uint32_t*)r);
+                            tc::tmem_ld_wait();
+                            pin(r);
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (j == hit) f[j] -= 1.f;
+                            for (int j = 0; j < 16; j += 2)
+                                unpair2(add2(pair2(v[i * 16 + j], v[i * 16 + j + 1]), pair2(r[j], r[j + 1])), v[i * 16 + j],
+                                        v[i * 16 + j + 1]);
                         }
-                        // a row that does not count gives zeros whatever its logits are
+                        give_back(acc);
+                    }
+                    if (!ok) break;
+                }
+                if (p.bias) {
 #pragma unroll
-                        for (int j = 0; j < 32; j++) f[j] = counts ? f[j] : 0.f;
-                        if (valid && n < p.ldp) {
-                            uint16_t* dst = p.prob + (size_t)row * p.ldp + n;
+                    for (int j = 0; j < 128; j += 8) {
+                        float b8[8];
+                        load8_f32(b8, bi + c_first + j);
 #pragma unroll
-                            for (int g = 0; g < 32; g += 16) {
-                                if (n + g >= p.ldp) break;
+                        for (int k = 0; k < 8; k += 2)
+                            unpair2(add2(pair2(v[j + k], v[j + k + 1]), pair2(b8[k], b8[k + 1])), v[j + k], v[j + k + 1]);
+                    }
+                }
+                const int columns = min(width, q.N - n_first);     // the rest lies past the vocabulary
+                if (columns < 128) {
+#pragma unroll
+                    for (int j = 0; j < 128; j++)
+                        if (j >= columns) v[j] = -INFINITY;
+                }
+                const int hit = label - n_first;          // the label's place among this warp's columns
+
+                if constexpr (EPI == kLse) {
+                    if (hit >= 0 && hit < columns) {
+#pragma unroll
+                        for (int j = 0; j < 128; j++)
+                            if (j == hit) p.label_logit[row] = v[j];
+                    }
+                    float m[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) m[j] = v[j];
+#pragma unroll
+                    for (int j = 4; j < 124; j += 8) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) m[k] = max3(m[k], v[j + 2 * k], v[j + 2 * k + 1]);
+                    }
+                    const float top = max3(max3(m[0], m[1], m[2]), m[3],
+                                           max3(fmaxf(v[124], v[125]), v[126], v[127]));
+                    float sum = 0.f;
+                    if (__all_sync(0xFFFFFFFFu, fabsf(top) < 1e30f)) {
+                        // one multiply-add: off by 2^-24 of |top| in the logarithm, as the logits themselves are
+                        const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(-top * LOG2E, -top * LOG2E);
+                        uint64_t s2[4] = {0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < 128; j += 2) {
+                            float a, b;
+                            unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
+                            s2[j / 2 % 4] = add2(s2[j / 2 % 4], pair2(ex2(a), ex2(b)));
+                        }
+                        float a, b;
+                        unpair2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), a, b);
+                        sum = a + b;
+                    } else {
+                        // Logits near the lowest fp32 value, whose product with log2 e overflows, or nothing but -inf: a
+                        // row whose entries are all taken out has sum 0 relative to 0.
+                        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                        for (int j = 0; j < 128; j++) sum += ex2((v[j] - ref) * LOG2E);
+                    }
+                    // the maximum and sum of this warp's columns, for each of its rows (kLse tiles are never cut in
+                    // two, so a 256-column block has these two entries)
+                    if (valid)
+                        p.partial[(size_t)(it.tile.n_blk * 2 + colgrp) * q.M + row] = make_float2(top, sum);
+                } else {
+                    // softmax(l) - onehot, times F16_GAIN (2^14, part of the exponent) for fp16
+                    const float gain = p.f16 ? F16_GAIN : 1.f, log2_gain = p.f16 ? 14.f : 0.f;
+                    if (__all_sync(0xFFFFFFFFu, fabsf(row_max) < 256.f)) {
+                        const float s1 = log2_gain - (row_max * LOG2E + log2_sum);     // off by 2^-15 of a probability at most
+                        const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(s1, s1);
+#pragma unroll
+                        for (int j = 0; j < 128; j += 2) {
+                            float a, b;
+                            unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
+                            v[j] = ex2(a);
+                            v[j + 1] = ex2(b);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 128; j++)
+                            v[j] = ex2(fmaf(v[j] - row_max, LOG2E, log2_gain - log2_sum));
+                    }
+                    if (hit >= 0 && hit < columns) {
+#pragma unroll
+                        for (int j = 0; j < 128; j++)
+                            if (j == hit) v[j] -= gain;
+                    }
+                    // a row that does not count gives zeros whatever its logits are
+                    const uint32_t keep = counts ? 0xFFFFFFFFu : 0u;
+                    if (valid) {
+                        uint16_t* dst = p.prob + (size_t)row * p.ldp + n_first;
+#pragma unroll
+                        for (int g = 0; g < 128; g += 16) {
+                            if (g < width && n_first + g < p.ldp) {
                                 u32x8 o;
 #pragma unroll
-                                for (int j = 0; j < 8; j++) {
-                                    const float a = f[g + 2 * j], b = f[g + 2 * j + 1];
-                                    o.v[j] = p.f16 ? pack_f16x2(a * F16_GAIN, b * F16_GAIN) : pack_bf16x2(a, b);
-                                }
+                                for (int j = 0; j < 8; j++)
+                                    o.v[j] = (p.f16 ? pack_f16x2(v[g + 2 * j], v[g + 2 * j + 1])
+                                                    : pack_bf16x2(v[g + 2 * j], v[g + 2 * j + 1])) & keep;
                                 stg_stream_256(dst + g, o);
                             }
                         }
-                        if (p.col_partial) {
-                            // Sums of 32 columns over the warp's 32 rows: at each step a lane keeps the half of
-                            // its columns that its lane bit names and adds its partner's; after five steps
-                            // lane l holds column l.
+                    }
+                    if (p.col_partial) {
+                        // Sums of 32 columns over the warp's 32 rows: at each step a lane keeps the half of its
+                        // columns that its lane bit names and adds its partner's; after five steps lane l holds
+                        // column l.
+#pragma unroll
+                        for (int c = 0; c < 128; c += 32) {
+                            if (c >= width) continue;
+                            float f[32];
+#pragma unroll
+                            for (int j = 0; j < 32; j++) f[j] = __uint_as_float(__float_as_uint(v[c + j]) & keep);
 #pragma unroll
                             for (int h = 16; h; h >>= 1) {
                                 const bool upper = (lane & h) != 0;
 #pragma unroll
                                 for (int j = 0; j < h; j++) {
-                                    const float keep = upper ? f[j + h] : f[j], give = upper ? f[j] : f[j + h];
-                                    f[j] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, h);
+                                    const float stay = upper ? f[j + h] : f[j], give = upper ? f[j] : f[j + h];
+                                    f[j] = stay + __shfl_xor_sync(0xFFFFFFFFu, give, h);
                                 }
                             }
-                            if (n + lane < p.ldp && m0 + quarter * 32 < q.M)
-                                p.col_partial[(size_t)((m0 >> 5) + quarter) * p.ldp + n + lane] = f[0];
+                            if (n_first + c + lane < p.ldp && m0 + quarter * 32 < q.M)
+                                p.col_partial[(size_t)((m0 >> 5) + quarter) * p.ldp + n_first + c + lane] = f[0];
                         }
-                    };
-                    uint32_t ra[32], rb[32];
-                    tc::tmem_ld_32x32(taddr + c_first, ra);
-#pragma unroll 1
-                    for (int c = c_first; c < c_end; c += 64) {
-                        tc::tmem_ld_wait();
-                        tc::tmem_ld_32x32(taddr + c + 32, rb);
-                        emit(ra, c);
-                        tc::tmem_ld_wait();
-                        if (c + 64 < c_end) tc::tmem_ld_32x32(taddr + c + 64, ra);
-                        emit(rb, c + 32);
                     }
-                    give_back(acc);
                 }
             }
         }
@@ -1014,7 +1062,7 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
         u.db = d_db ? d_db + v0 : nullptr;
         u.db_n = (int)nv;
         u.groups = (int)((M + 31) / 32);
-        u.db_scale = grad_scale;
+        u.db_scale = u.scale;
         Problem dx = {}, dw = {};
         dx.M = (int)M;
         dx.N = dw.N = (int)K;
@@ -1054,7 +1102,7 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
         if (n > 1) u.q[swap ? 0 : 1] = *wanted[1];
         const bool first_dw = n > 0 && wanted[swap ? 1 : 0] == &dw;
         if (n == 0) {
-            s = launch_after(bias_grad_kernel, (nv + 31) / 32, 256, 0, st, u.db, cols, u.groups, u.ldp, u.db_n, grad_scale,
+            s = launch_after(bias_grad_kernel, (nv + 31) / 32, 256, 0, st, u.db, cols, u.groups, u.ldp, u.db_n, u.db_scale,
                              count);
         } else {
             s = first_dw ? launch_gemm<kSum>(u, g_mn, x_mn, g_k, w_mn, device, st)
