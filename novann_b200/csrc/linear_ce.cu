@@ -48,7 +48,7 @@ struct Problem : LinearParams {
 
 struct CeParams {
     Problem q[2];                // kSum: up to two contractions in one launch, the longer items first
-    int f16;                     // operands are fp16 (else bf16)
+    int lead;                    // see nth_item
     int* status;
     // kLse, kProb
     const float* bias;
@@ -150,13 +150,34 @@ __device__ __forceinline__ Item item_of(const CeParams& p, int t) {
     return it;
 }
 
+// The n-th item of a pair, or -1.  The first contraction's items are dealt out in turn; the pairs that got one less then take
+// `lead` of the second's each (as many as last as long as the item that they did not get), and what is left is
+// dealt out to all.
+__device__ __forceinline__ int nth_item(const CeParams& p, int pair, int num_pairs, int n) {
+    const int n0 = p.q[0].num_items, n1 = p.q[1].num_items, r0 = n0 % num_pairs;
+    const int mine = n0 / num_pairs + (pair < r0);
+    if (n < mine) return pair + n * num_pairs;
+    n -= mine;
+    const int idle = num_pairs - r0;
+    int i;
+    if (pair >= r0 && n < p.lead) i = pair - r0 + n * idle;
+    else i = idle * p.lead + pair + (pair >= r0 ? n - p.lead : n) * num_pairs;
+    return i < n1 ? n0 + i : -1;
+}
+
 // kLse keeps at most this many k-blocks (1024 of K) in one TMEM accumulator: the tensor core cuts off where it adds, by
 // up to a step of the running sum each time, and over 4096 of K the logits were off by 1e-6 of themselves, all
 // towards zero.  The parts are joined in registers; MMAs and epilogue alternate between the two accumulators as
 // they do between tiles.
 constexpr int PART_KB = 16;
 
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    return F16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+}
+
 // 32 fp32 sums of one row (columns n ...): to the fp32 buffer, or scaled to the final type
+template <bool F16>
 __device__ __forceinline__ void store_sum(const Problem& p, int out_type, const uint32_t* r, size_t at, int n, int split,
                                           float s) {
     if (p.out == nullptr || out_type == NVQ_F32) {
@@ -183,8 +204,7 @@ __device__ __forceinline__ void store_sum(const Problem& p, int out_type, const 
             u32x8 o;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float a = __uint_as_float(r[g + 2 * j]) * s, b = __uint_as_float(r[g + 2 * j + 1]) * s;
-                o.v[j] = out_type == NVQ_F16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+                o.v[j] = pack16<F16>(__uint_as_float(r[g + 2 * j]) * s, __uint_as_float(r[g + 2 * j + 1]) * s);
             }
             if (p.vec32 && n + g + 16 <= p.N) {
                 stg_stream_256(dst + g, o);
@@ -197,7 +217,8 @@ __device__ __forceinline__ void store_sum(const Problem& p, int out_type, const 
 }
 
 // kLse, kProb: both operands with the contraction contiguous.  kSum: B with N contiguous, A as Problem::a_mn says.
-template <int EPI>
+// F16: operands (and 16-bit results) are fp16, else bf16.
+template <int EPI, bool F16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
                const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
@@ -210,7 +231,6 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_ctarank();
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-    const int num_items = p.q[0].num_items + p.q[1].num_items;
     volatile int* abort_flag = &sh->abort_flag;
     // accumulators: two of 256 columns
     auto acc_of = [&](int n, uint32_t& acc, uint32_t& acc_phase) { acc = n & 1; acc_phase = (n >> 1) & 1; };
@@ -250,7 +270,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (int t = pair; t < num_items && ok; t += num_pairs) {
+            for (int i = 0, t; ok && (t = nth_item(p, pair, num_pairs, i)) >= 0; i++) {
                 const Item it = item_of(p, t);
                 const CUtensorMap* map_a = it.second ? &map_a1 : &map_a0;
                 const CUtensorMap* map_b = it.second ? &map_b1 : &map_b0;
@@ -289,8 +309,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
             uint32_t stage = 0, phase = 0;
             bool ok = true, ready = false;
             int n = 0;
-            const uint32_t fmt = p.f16 ? 0u : 1u;
-            for (int t = pair; t < num_items && ok; t += num_pairs) {
+            constexpr uint32_t fmt = F16 ? 0u : 1u;
+            for (int i = 0, t; ok && (t = nth_item(p, pair, num_pairs, i)) >= 0; i++) {
                 const Item it = item_of(p, t);
                 const bool a_mn = EPI == kSum && it.q->a_mn;
                 const uint32_t idesc = tc::idesc_f16(BM, it.tile.is_half ? BN / 2 : BN, fmt, fmt) |
@@ -381,7 +401,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
             }
         }
 
-        for (int t = pair, n_tile = 0; t < num_items && ok; t += num_pairs, n_tile++) {
+        for (int n_tile = 0, t; ok && (t = nth_item(p, pair, num_pairs, n_tile)) >= 0; n_tile++) {
             const Item it = item_of(p, t);
             const Problem& q = *it.q;
             const int bn = it.tile.is_half ? BN / 2 : BN;
@@ -410,7 +430,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                             for (int j = 0; j < 8; j++) r[g + j] = __float_as_uint(__uint_as_float(r[g + j]) + a[j]);
                         }
                     }
-                    store_sum(q, p.out_type, r, at, n, it.split, out_scale);
+                    store_sum<F16>(q, p.out_type, r, at, n, it.split, out_scale);
                 };
                 // a chunk is loaded from TMEM while the one before it is worked on
                 uint32_t ra[32], rb[32];
@@ -511,48 +531,46 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                     }
                     const float top = max3(max3(m[0], m[1], m[2]), m[3],
                                            max3(fmaxf(v[124], v[125]), v[126], v[127]));
-                    float sum = 0.f;
-                    if (__all_sync(0xFFFFFFFFu, fabsf(top) < 1e30f)) {
-                        // one multiply-add: off by 2^-24 of |top| in the logarithm, as the logits themselves are
-                        const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(-top * LOG2E, -top * LOG2E);
-                        uint64_t s2[4] = {0, 0, 0, 0};
-#pragma unroll
-                        for (int j = 0; j < 128; j += 2) {
-                            float a, b;
-                            unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
-                            s2[j / 2 % 4] = add2(s2[j / 2 % 4], pair2(ex2(a), ex2(b)));
-                        }
-                        float a, b;
-                        unpair2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), a, b);
-                        sum = a + b;
-                    } else {
+                    // exp(l - top) by one multiply-add, off by 2^-24 of |top| in the exponent, as the logits are
+                    float s1 = -top * LOG2E;
+                    if (!__all_sync(0xFFFFFFFFu, fabsf(top) < 1e30f)) {
                         // Logits near the lowest fp32 value, whose product with log2 e overflows, or nothing but -inf: a
                         // row whose entries are all taken out has sum 0 relative to 0.
                         const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                        for (int j = 0; j < 128; j++) sum += ex2((v[j] - ref) * LOG2E);
+                        for (int j = 0; j < 128; j++) v[j] -= ref;
+                        s1 = 0.f;
                     }
+                    const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(s1, s1);
+                    uint64_t s2[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 128; j += 2) {
+                        float a, b;
+                        unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
+                        s2[j / 2 % 4] = add2(s2[j / 2 % 4], pair2(ex2(a), ex2(b)));
+                    }
+                    float s_even, s_odd;
+                    unpair2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), s_even, s_odd);
                     // the maximum and sum of this warp's columns, for each of its rows (kLse tiles are never cut in
                     // two, so a 256-column block has these two entries)
                     if (valid)
-                        p.partial[(size_t)(it.tile.n_blk * 2 + colgrp) * q.M + row] = make_float2(top, sum);
+                        p.partial[(size_t)(it.tile.n_blk * 2 + colgrp) * q.M + row] = make_float2(top, s_even + s_odd);
                 } else {
                     // softmax(l) - onehot, times F16_GAIN (2^14, part of the exponent) for fp16
-                    const float gain = p.f16 ? F16_GAIN : 1.f, log2_gain = p.f16 ? 14.f : 0.f;
-                    if (__all_sync(0xFFFFFFFFu, fabsf(row_max) < 256.f)) {
-                        const float s1 = log2_gain - (row_max * LOG2E + log2_sum);     // off by 2^-15 of a probability at most
-                        const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(s1, s1);
+                    constexpr float gain = F16 ? F16_GAIN : 1.f, log2_gain = F16 ? 14.f : 0.f;
+                    float s1 = log2_gain - (row_max * LOG2E + log2_sum);      // off by 2^-15 of a probability at most
+                    if (!__all_sync(0xFFFFFFFFu, fabsf(row_max) < 256.f)) {
 #pragma unroll
-                        for (int j = 0; j < 128; j += 2) {
-                            float a, b;
-                            unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
-                            v[j] = ex2(a);
-                            v[j + 1] = ex2(b);
-                        }
-                    } else {
+                        for (int j = 0; j < 128; j++) v[j] -= row_max;
+                        s1 = log2_gain - log2_sum;
+                    }
+                    const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(s1, s1);
 #pragma unroll
-                        for (int j = 0; j < 128; j++)
-                            v[j] = ex2(fmaf(v[j] - row_max, LOG2E, log2_gain - log2_sum));
+                    for (int j = 0; j < 128; j += 2) {
+                        float a, b;
+                        unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
+                        v[j] = ex2(a);
+                        v[j + 1] = ex2(b);
                     }
                     if (hit >= 0 && hit < columns) {
 #pragma unroll
@@ -569,8 +587,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                                 u32x8 o;
 #pragma unroll
                                 for (int j = 0; j < 8; j++)
-                                    o.v[j] = (p.f16 ? pack_f16x2(v[g + 2 * j], v[g + 2 * j + 1])
-                                                    : pack_bf16x2(v[g + 2 * j], v[g + 2 * j + 1])) & keep;
+                                    o.v[j] = pack16<F16>(v[g + 2 * j], v[g + 2 * j + 1]) & keep;
                                 stg_stream_256(dst + g, o);
                             }
                         }
@@ -785,12 +802,13 @@ nvq_status launch_after(void (*kernel)(KArgs...), size_t grid, int threads, int 
     return NVQ_OK;
 }
 
-template <int EPI>
-nvq_status launch_gemm(CeParams& p, const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
+template <int EPI, bool F16>
+nvq_status launch_gemm_typed(CeParams& p, const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
                        const CUtensorMap& b1, int device, cudaStream_t st) {
     static std::atomic<bool> attr_set[64];   // per device; setting the attribute twice is harmless
     if (!attr_set[device]) {
-        NVQ_CUDA(cudaFuncSetAttribute(ce_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+        NVQ_CUDA(cudaFuncSetAttribute(ce_gemm_kernel<EPI, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      SMEM_BYTES));
         attr_set[device] = true;
     }
     nvq_status s = nvq_status_word(device, &p.status);
@@ -799,7 +817,10 @@ nvq_status launch_gemm(CeParams& p, const CUtensorMap& a0, const CUtensorMap& b0
     for (Problem& q : p.q) {
         q.m_blocks = (q.M + BM - 1) / BM;
         q.n_blocks = (q.N + BN - 1) / BN;
-        q.group_m = 8;
+        // row blocks walked together: a panel of about 32 MB of A stays in L2 while B streams past it
+        const int kb = q.splits > 1 ? q.kb_per : (q.K + BK - 1) / BK;
+        const int most = (int)((32u << 20) / (BM * BK * 2) / (kb ? kb : 1));
+        q.group_m = most < 4 ? 4 : (most > 16 ? 16 : most);
         q.num_big = q.num_items = q.m_blocks * q.n_blocks * q.splits;
     }
     // a partial last wave that would occupy at most half of the pairs is cut into half-width tiles
@@ -811,7 +832,19 @@ nvq_status launch_gemm(CeParams& p, const CUtensorMap& a0, const CUtensorMap& b0
     }
     const int items = p.q[0].num_items + p.q[1].num_items;
     const int used = items < pairs ? items : pairs;
-    return launch_after(ce_gemm_kernel<EPI>, 2 * (size_t)used, THREADS, SMEM_BYTES, st, a0, b0, a1, b1, p);
+    p.lead = 0;
+    if (p.q[1].num_items && p.q[0].num_items % used) {
+        const int kb0 = p.q[0].splits > 1 ? p.q[0].kb_per : (p.q[0].K + BK - 1) / BK;
+        const int kb1 = p.q[1].splits > 1 ? p.q[1].kb_per : (p.q[1].K + BK - 1) / BK;
+        p.lead = (kb0 + kb1 / 2) / kb1;
+    }
+    return launch_after(ce_gemm_kernel<EPI, F16>, 2 * (size_t)used, THREADS, SMEM_BYTES, st, a0, b0, a1, b1, p);
+}
+template <int EPI>
+nvq_status launch_gemm(CeParams& p, bool f16, const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
+                       const CUtensorMap& b1, int device, cudaStream_t st) {
+    return f16 ? launch_gemm_typed<EPI, true>(p, a0, b0, a1, b1, device, st)
+               : launch_gemm_typed<EPI, false>(p, a0, b0, a1, b1, device, st);
 }
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
@@ -965,12 +998,11 @@ extern "C" nvq_status nvq_linear_ce_fwd(float* d_loss_count, float* d_row_loss, 
     p.q[0].N = (int)V;
     p.q[0].K = (int)K;
     p.q[0].splits = 1;
-    p.f16 = dtype == NVQ_F16;
     p.bias = d_bias;
     p.labels = d_labels;
     p.partial = partial;
     p.label_logit = logit;
-    s = launch_gemm<kLse>(p, a, b, a, b, device, st);
+    s = launch_gemm<kLse>(p, dtype == NVQ_F16, a, b, a, b, device, st);
     if (s != NVQ_OK) return s;
     // up to eight partial sums a row: a warp adds up 32 rows by itself; more: the whole block does
     const int slots = 2 * p.q[0].n_blocks, mean = reduction == NVQ_REDUCE_MEAN;
@@ -1018,6 +1050,7 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
     float* sum = (float*)(ws + sp.prob + sp.cols);
     char* parts = ws + sp.prob + sp.cols + sp.sum;
     const float* count = reduction == NVQ_REDUCE_MEAN ? d_loss_count + 1 : nullptr;
+    const bool f16 = dtype == NVQ_F16;
     const size_t piece = piece_of(M, V);
     CUtensorMap x_k, x_mn;      // X with the contraction along its rows, and across them
     s = nvq_make_tmap_2d(&x_k, d_x, M, K, 128, BK, 2, 1);
@@ -1038,7 +1071,6 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
         p.q[0].N = (int)nv;
         p.q[0].K = (int)K;
         p.q[0].splits = 1;
-        p.f16 = dtype == NVQ_F16;
         p.bias = d_bias ? d_bias + v0 : nullptr;
         p.labels = d_labels;
         p.stats = d_row_stats;
@@ -1048,14 +1080,13 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
         p.prob = prob;
         p.ldp = (int)ld;
         p.col_partial = d_db ? cols : nullptr;
-        s = launch_gemm<kProb>(p, x_k, w_k, x_k, w_k, device, st);
+        s = launch_gemm<kProb>(p, f16, x_k, w_k, x_k, w_k, device, st);
         if (s != NVQ_OK) return s;
 
         // dX and dW of the piece in one launch, and db beside them
         CeParams u = {};
-        u.f16 = p.f16;
         u.out_type = grad_dtype;
-        u.scale = grad_scale / (p.f16 ? F16_GAIN : 1.f);
+        u.scale = grad_scale / (f16 ? F16_GAIN : 1.f);
         u.count = count;
         u.col_partial = cols;
         u.ldp = (int)ld;
@@ -1105,8 +1136,8 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
             s = launch_after(bias_grad_kernel, (nv + 31) / 32, 256, 0, st, u.db, cols, u.groups, u.ldp, u.db_n, u.db_scale,
                              count);
         } else {
-            s = first_dw ? launch_gemm<kSum>(u, g_mn, x_mn, g_k, w_mn, device, st)
-                         : launch_gemm<kSum>(u, g_k, w_mn, g_mn, x_mn, device, st);
+            s = first_dw ? launch_gemm<kSum>(u, f16, g_mn, x_mn, g_k, w_mn, device, st)
+                         : launch_gemm<kSum>(u, f16, g_k, w_mn, g_mn, x_mn, device, st);
         }
         if (s != NVQ_OK) return s;
         for (int i = 0; i < n; i++) {
