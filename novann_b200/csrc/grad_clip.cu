@@ -3,8 +3,8 @@
 //   norm = sqrt(sum over tensors, sum over elements of g^2)
 //   coef = 1 if norm <= max_norm, else max_norm / norm;   out = g * coef
 //
-// Both kernels walk one list of chunks of CHUNK elements; a chunk lies in one tensor and belongs to
-// a fixed block, so that the sum is always added in the same order (equal inputs give equal bits)
+// Both kernels walk one list of chunks of 16 KB; a chunk lies in one tensor and belongs to a fixed block (the
+// blocks take neighbouring chunks at the same time, which is what DRAM likes best), so that the sum is always added in the same order (equal inputs give equal bits)
 // and nothing is counted by atomics.  The tensor list travels in the kernel's parameters: no copy
 // to the device, and a captured graph keeps its own.  Squares are added in fp64 (one conversion and
 // one fused multiply-add per element, which the memory rate leaves room for): no gradient that fits
@@ -14,7 +14,7 @@
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int CHUNK = 4096;            // elements: 16 per thread, four 16-byte loads of fp32
+constexpr int CHUNK_BYTES = 16384;     // 64 per thread: two 32-byte loads
 constexpr int BLOCKS_PER_SM = 8;
 constexpr int MAX_BLOCKS = 148 * BLOCKS_PER_SM;
 
@@ -25,7 +25,7 @@ struct TensorList {
     unsigned long long count[NT];
     uint32_t first[NT + 1];     // chunk number at which the tensor starts
     uint8_t dtype[NT];
-    uint8_t vec[NT];            // 16-byte packets are aligned in src (and dst)
+    uint8_t vec[NT];            // src and dst lie alike within 32 bytes
     int n;
 };
 
@@ -52,30 +52,59 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
     return s;
 }
 
-// sum of squares of n <= CHUNK elements at p, this thread's share
+__host__ __device__ constexpr int elem_size(int dt) { return dt == NVQ_F64 ? 8 : (dt == NVQ_F32 ? 4 : 2); }
+__host__ __device__ constexpr int chunk_elems(int dt) { return CHUNK_BYTES / elem_size(dt); }
+
+__device__ __forceinline__ u32x8 ld256(const void* p) {
+    u32x8 r;
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]), "=r"(r.v[4]), "=r"(r.v[5]), "=r"(r.v[6]),
+                   "=r"(r.v[7])
+                 : "l"(p)
+                 : "memory");
+    return r;
+}
+
+// Calls wide(i) for every 32-byte packet of a chunk of n elements at p (pairs(i, i + THREADS) where both exist) and
+// one(k) for the elements before the first and after the last of them.
+template <int SIZE, typename Pairs, typename Wide, typename One>
+__device__ __forceinline__ void walk(const void* p, int n, bool vec, Pairs pairs, Wide wide, One one) {
+    constexpr int V = 32 / SIZE;
+    const int head = vec ? min(n, (int)((32 - ((uintptr_t)p & 31)) & 31) / SIZE) : n;
+    const int packets = (n - head) / V, tail = head + packets * V;
+    int i = threadIdx.x;
+    for (; i + THREADS < packets; i += 2 * THREADS) pairs(head, i, i + THREADS);
+    if (i < packets) wide(head, i);
+    for (int k = threadIdx.x; k < head; k += THREADS) one(k);
+    for (int k = tail + threadIdx.x; k < n; k += THREADS) one(k);
+}
+
+// sum of squares of a chunk of n elements at p, this thread's share
 template <int DT>
-__device__ __forceinline__ double chunk_squares(const void* p, int n, bool vec) {
+__device__ __forceinline__ double chunk_squares(const char* p, int n, bool vec) {
     using E = Elem<DT>;
     double s = 0.0;
-    if (vec && n == CHUNK) {
-        constexpr int V = 16 / E::SIZE, ROUNDS = CHUNK / (V * THREADS);
-        Packet<DT, V> q[ROUNDS];
+    auto add = [&](const u32x8& q) {
 #pragma unroll
-        for (int i = 0; i < ROUNDS; i++)
-            q[i].load((const char*)p + (size_t)(i * THREADS + threadIdx.x) * 16);
+        for (int w = 0; w < 8; w++) {
+            float f[2];
+            E::widen(q.v[w], f);
 #pragma unroll
-        for (int i = 0; i < ROUNDS; i++) {
-            float f[V];
-            q[i].widen(f);
-#pragma unroll
-            for (int j = 0; j < V; j++) s = fma((double)f[j], (double)f[j], s);
+            for (int j = 0; j < E::PER_WORD; j++) s = fma((double)f[j], (double)f[j], s);
         }
-    } else {
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            const double f = (double)E::load((const char*)p + (size_t)i * E::SIZE);
+    };
+    walk<E::SIZE>(
+        p, n, vec,
+        [&](int h, int i, int k) {
+            const u32x8 a = ld256(p + h * E::SIZE + i * 32), b = ld256(p + h * E::SIZE + k * 32);
+            add(a);
+            add(b);
+        },
+        [&](int h, int i) { add(ld256(p + h * E::SIZE + i * 32)); },
+        [&](int k) {
+            const double f = (double)E::load(p + k * E::SIZE);
             s = fma(f, f, s);
-        }
-    }
+        });
     return s;
 }
 __device__ __forceinline__ double chunk_squares_f64(const double* p, int n) {
@@ -84,29 +113,23 @@ __device__ __forceinline__ double chunk_squares_f64(const double* p, int n) {
     return s;
 }
 
-__host__ __device__ constexpr int elem_size(int dt) { return dt == NVQ_F64 ? 8 : (dt == NVQ_F32 ? 4 : 2); }
-
 // partial[block] = (add ? partial[block] : 0) + the block's share of the sum of squares
 template <int NT>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM)
-square_sum_kernel(const __grid_constant__ TensorList<NT> L, double* __restrict__ partial, uint32_t chunks,
-                  uint32_t per_block, int add) {
+square_sum_kernel(const __grid_constant__ TensorList<NT> L, double* __restrict__ partial, uint32_t chunks, int add) {
     __shared__ double sh[THREADS / 32];
-    const uint32_t c0 = blockIdx.x * per_block, c1 = min(chunks, c0 + per_block);
     double s = 0.0;
-    if (c0 < c1) {
-        int t = find_tensor(L, c0);
-        for (uint32_t c = c0; c < c1; c++) {
-            while (c >= L.first[t + 1]) t++;
-            const size_t at = (size_t)(c - L.first[t]) * CHUNK;
-            const int n = (int)min((unsigned long long)CHUNK, L.count[t] - at);
-            const int dt = L.dtype[t];
-            const void* p = (const char*)L.src[t] + at * elem_size(dt);
-            if (dt == NVQ_F32) s += chunk_squares<NVQ_F32>(p, n, L.vec[t]);
-            else if (dt == NVQ_BF16) s += chunk_squares<NVQ_BF16>(p, n, L.vec[t]);
-            else if (dt == NVQ_F16) s += chunk_squares<NVQ_F16>(p, n, L.vec[t]);
-            else s += chunk_squares_f64((const double*)p, n);
-        }
+    int t = 0;
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        if (c >= L.first[t + 1]) t = find_tensor(L, c);
+        const int dt = L.dtype[t];
+        const size_t at = (size_t)(c - L.first[t]) * chunk_elems(dt);
+        const int n = (int)min((unsigned long long)chunk_elems(dt), L.count[t] - at);
+        const char* p = (const char*)L.src[t] + at * elem_size(dt);
+        if (dt == NVQ_F32) s += chunk_squares<NVQ_F32>(p, n, L.vec[t]);
+        else if (dt == NVQ_BF16) s += chunk_squares<NVQ_BF16>(p, n, L.vec[t]);
+        else if (dt == NVQ_F16) s += chunk_squares<NVQ_F16>(p, n, L.vec[t]);
+        else s += chunk_squares_f64((const double*)p, n);
     }
     s = block_sum(s, sh);
     if (threadIdx.x == 0) partial[blockIdx.x] = (add ? partial[blockIdx.x] : 0.0) + s;
@@ -136,36 +159,37 @@ norm_kernel(float* __restrict__ out, const double* __restrict__ partial, int blo
 }
 
 template <int DT>
-__device__ __forceinline__ void chunk_scale(void* d, const void* p, int n, bool vec, float coef) {
+__device__ __forceinline__ void chunk_scale(char* d, const char* p, int n, bool vec, float coef) {
     using E = Elem<DT>;
-    if (vec && n == CHUNK) {
-        constexpr int V = 16 / E::SIZE, ROUNDS = CHUNK / (V * THREADS);
-        Packet<DT, V> q[ROUNDS];
+    auto cut = [&](u32x8 q, char* to) {
 #pragma unroll
-        for (int i = 0; i < ROUNDS; i++)
-            q[i].load_once((const char*)p + (size_t)(i * THREADS + threadIdx.x) * 16);
+        for (int w = 0; w < 8; w++) {
+            float f[2];
+            E::widen(q.v[w], f);
 #pragma unroll
-        for (int i = 0; i < ROUNDS; i++) {
-            float f[V];
-            q[i].widen(f);
-#pragma unroll
-            for (int j = 0; j < V; j++) f[j] *= coef;
-            q[i].narrow(f);
-            q[i].store((char*)d + (size_t)(i * THREADS + threadIdx.x) * 16);
+            for (int j = 0; j < E::PER_WORD; j++) f[j] *= coef;
+            q.v[w] = E::narrow(f);
         }
-    } else {
-        for (int i = threadIdx.x; i < n; i += THREADS)
-            E::store((char*)d + (size_t)i * E::SIZE, E::load((const char*)p + (size_t)i * E::SIZE) * coef);
-    }
+        stg_stream_256(to, q);
+    };
+    walk<E::SIZE>(
+        p, n, vec,
+        [&](int h, int i, int k) {
+            const u32x8 a = ld256(p + h * E::SIZE + i * 32), b = ld256(p + h * E::SIZE + k * 32);
+            cut(a, d + h * E::SIZE + i * 32);
+            cut(b, d + h * E::SIZE + k * 32);
+        },
+        [&](int h, int i) { cut(ld256(p + h * E::SIZE + i * 32), d + h * E::SIZE + i * 32); },
+        [&](int k) { E::store(d + k * E::SIZE, E::load(p + k * E::SIZE) * coef); });
 }
 
 // Every block adds the (at most 1184) partial sums up again, which costs less than a launch between
-// the two kernels.  A block walks its chunks backwards: the ones that the first kernel read last are
-// those that still lie in L2.
+// the two kernels.  The chunks are walked backwards: the ones that the first kernel read last are those that
+// still lie in L2.
 template <int NT>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM)
 clip_kernel(const __grid_constant__ TensorList<NT> L, float* __restrict__ out, const double* __restrict__ partial,
-            int blocks, double max_norm, uint32_t chunks, uint32_t per_block) {
+            int blocks, double max_norm, uint32_t chunks) {
     __shared__ double sh[THREADS / 32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const double norm = total_norm(partial, blocks, sh);
@@ -175,16 +199,15 @@ clip_kernel(const __grid_constant__ TensorList<NT> L, float* __restrict__ out, c
         out[0] = (float)norm;
         out[1] = coef;
     }
-    const uint32_t c0 = blockIdx.x * per_block, c1 = min(chunks, c0 + per_block);
-    if (c0 >= c1) return;
-    int t = find_tensor(L, c1 - 1);
-    for (uint32_t c = c1; c-- > c0;) {
-        while (c < L.first[t]) t--;
-        const size_t at = (size_t)(c - L.first[t]) * CHUNK;
-        const int n = (int)min((unsigned long long)CHUNK, L.count[t] - at);
+    int t = L.n - 1;
+    for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
+        const uint32_t c = chunks - 1 - k;
+        if (c < L.first[t]) t = find_tensor(L, c);
         const int dt = L.dtype[t];
-        const void* p = (const char*)L.src[t] + at * elem_size(dt);
-        void* d = (char*)L.dst[t] + at * elem_size(dt);
+        const size_t at = (size_t)(c - L.first[t]) * chunk_elems(dt);
+        const int n = (int)min((unsigned long long)chunk_elems(dt), L.count[t] - at);
+        const char* p = (const char*)L.src[t] + at * elem_size(dt);
+        char* d = (char*)L.dst[t] + at * elem_size(dt);
         if (coef64 == 1.0 && p == d) continue;      // in place and nothing to cut
         if (dt == NVQ_F32) chunk_scale<NVQ_F32>(d, p, n, L.vec[t], coef);
         else if (dt == NVQ_BF16) chunk_scale<NVQ_BF16>(d, p, n, L.vec[t], coef);
@@ -217,14 +240,14 @@ size_t fill(TensorList<NT>& L, const void* const* src, void* const* dst, const s
     size_t t = begin;
     for (; t < n && L.n < NT; t++) {
         if (counts[t] == 0) continue;
-        const uint64_t c = (counts[t] + CHUNK - 1) / CHUNK;
+        const uint64_t each = chunk_elems(dtypes[t]), c = (counts[t] + each - 1) / each;
         if (total + c > 0x7FFFFFFFull) break;
         L.src[L.n] = src[t];
         L.dst[L.n] = dst ? dst[t] : const_cast<void*>(src[t]);
         L.count[L.n] = counts[t];
         L.first[L.n] = (uint32_t)total;
         L.dtype[L.n] = (uint8_t)dtypes[t];
-        L.vec[L.n] = nvq_aligned(src[t], 16) && (!dst || nvq_aligned(dst[t], 16));
+        L.vec[L.n] = !dst || ((uintptr_t)src[t] & 31) == ((uintptr_t)dst[t] & 31);
         total += c;
         L.n++;
     }
@@ -233,13 +256,7 @@ size_t fill(TensorList<NT>& L, const void* const* src, void* const* dst, const s
     return t;
 }
 
-struct Split { int grid; uint32_t per_block; };
-Split split_chunks(uint32_t chunks) {
-    Split s;
-    s.per_block = (chunks + MAX_BLOCKS - 1) / MAX_BLOCKS;
-    s.grid = (int)((chunks + s.per_block - 1) / s.per_block);
-    return s;
-}
+int blocks_for(uint32_t chunks) { return chunks < (uint32_t)MAX_BLOCKS ? (int)chunks : MAX_BLOCKS; }
 
 // Few tensors take the short list (2 KB of parameters); more take lists of up to 1024.
 constexpr int SHORT_LIST = 64, LONG_LIST = 1000;
@@ -253,14 +270,13 @@ nvq_status run_lists(float* d_out, void* const* dst, const void* const* src, con
     for (size_t t = 0; t < n;) {
         t = fill(L, src, dst, counts, dtypes, t, n, &chunks);
         if (chunks == 0) break;
-        const Split s = split_chunks(chunks);
+        const int grid = blocks_for(chunks);
         // a later list adds to the partial sums of the first ones, block by block
-        const int old = blocks < s.grid ? blocks : s.grid;
-        if (blocks && old < s.grid)
-            NVQ_CUDA(cudaMemsetAsync(partial + old, 0, (s.grid - old) * sizeof(double), st));
-        square_sum_kernel<NT><<<s.grid, THREADS, 0, st>>>(L, partial, chunks, s.per_block, blocks != 0);
+        if (blocks && blocks < grid)
+            NVQ_CUDA(cudaMemsetAsync(partial + blocks, 0, (grid - blocks) * sizeof(double), st));
+        square_sum_kernel<NT><<<grid, THREADS, 0, st>>>(L, partial, chunks, blocks != 0);
         NVQ_LAUNCHED();
-        if (s.grid > blocks) blocks = s.grid;
+        if (grid > blocks) blocks = grid;
     }
     if (!clip || blocks == 0) {
         launch_after(norm_kernel, 1, st, d_out, (const double*)partial, blocks, max_norm);
@@ -270,9 +286,7 @@ nvq_status run_lists(float* d_out, void* const* dst, const void* const* src, con
     for (size_t t = 0; t < n;) {
         t = fill(L, src, dst, counts, dtypes, t, n, &chunks);
         if (chunks == 0) break;
-        const Split s = split_chunks(chunks);
-        launch_after(clip_kernel<NT>, s.grid, st, L, d_out, (const double*)partial, blocks, max_norm, chunks,
-                     s.per_block);
+        launch_after(clip_kernel<NT>, blocks_for(chunks), st, L, d_out, (const double*)partial, blocks, max_norm, chunks);
         NVQ_LAUNCHED();
     }
     return NVQ_OK;
