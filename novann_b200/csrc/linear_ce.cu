@@ -176,42 +176,35 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     return F16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
 }
 
-// 32 fp32 sums of one row (columns n ...): to the fp32 buffer, or scaled to the final type
-template <bool F16>
-__device__ __forceinline__ void store_sum(const Problem& p, int out_type, const uint32_t* r, size_t at, int n, int split,
-                                          float s) {
-    if (p.out == nullptr || out_type == NVQ_F32) {
-        float* dst = p.out ? (float*)p.out + at : p.sum + (size_t)split * p.M * p.N + at;
-        const bool wide = p.out == nullptr || p.vec32;
+// `columns` of one row's sums, times s; wide: dst lies on a 32-byte boundary, else on a 16-byte one
+__device__ __forceinline__ void store_f32(float* dst, const float (&v)[128], int columns, float s, bool wide) {
 #pragma unroll
-        for (int g = 0; g < 32; g += 8) {
-            if (n + g >= p.N) break;
-            u32x8 o;
+    for (int g = 0; g < 128; g += 8) {
+        if (g >= columns) break;
+        u32x8 o;
 #pragma unroll
-            for (int j = 0; j < 8; j++) o.v[j] = __float_as_uint(__uint_as_float(r[g + j]) * s);
-            if (wide) {
-                stg_stream_256(dst + g, o);
-            } else {
-                stg_stream_128(dst + g, make_uint4(o.v[0], o.v[1], o.v[2], o.v[3]));
-                stg_stream_128(dst + g + 4, make_uint4(o.v[4], o.v[5], o.v[6], o.v[7]));
-            }
+        for (int j = 0; j < 8; j++) o.v[j] = __float_as_uint(v[g + j] * s);
+        if (wide) {
+            stg_stream_256(dst + g, o);
+        } else {
+            stg_stream_128(dst + g, make_uint4(o.v[0], o.v[1], o.v[2], o.v[3]));
+            stg_stream_128(dst + g + 4, make_uint4(o.v[4], o.v[5], o.v[6], o.v[7]));
         }
-    } else {
-        uint16_t* dst = (uint16_t*)p.out + at;
+    }
+}
+template <bool F16>
+__device__ __forceinline__ void store_16(uint16_t* dst, const float (&v)[128], int columns, float s, bool wide) {
 #pragma unroll
-        for (int g = 0; g < 32; g += 16) {
-            if (n + g >= p.N) break;
-            u32x8 o;
+    for (int g = 0; g < 128; g += 16) {
+        if (g >= columns) break;
+        u32x8 o;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                o.v[j] = pack16<F16>(__uint_as_float(r[g + 2 * j]) * s, __uint_as_float(r[g + 2 * j + 1]) * s);
-            }
-            if (p.vec32 && n + g + 16 <= p.N) {
-                stg_stream_256(dst + g, o);
-            } else {
-                stg_stream_128(dst + g, make_uint4(o.v[0], o.v[1], o.v[2], o.v[3]));
-                if (n + g + 16 <= p.N) stg_stream_128(dst + g + 8, make_uint4(o.v[4], o.v[5], o.v[6], o.v[7]));
-            }
+        for (int j = 0; j < 8; j++) o.v[j] = pack16<F16>(v[g + 2 * j] * s, v[g + 2 * j + 1] * s);
+        if (wide && g + 16 <= columns) {
+            stg_stream_256(dst + g, o);
+        } else {
+            stg_stream_128(dst + g, make_uint4(o.v[0], o.v[1], o.v[2], o.v[3]));
+            if (g + 16 <= columns) stg_stream_128(dst + g + 8, make_uint4(o.v[4], o.v[5], o.v[6], o.v[7]));
         }
     }
 }
@@ -362,6 +355,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
         auto take = [&](uint32_t& taddr) -> uint32_t {
             uint32_t acc, acc_phase;
             acc_of(n_acc++, acc, acc_phase);
+            __syncwarp();            // rows past the end have skipped the stores of the tile before
             ok = tc::mbar_wait(tc::smem_u32(&sh->tmem_full[acc]), acc_phase, abort_flag, ERR_EPILOGUE);
             ok = epilogue_all<32 * EPI_WARPS>(ok);
             tc::tc_fence_after();
@@ -409,42 +403,46 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
             const int n0 = it.tile.n_blk * BN + it.tile.half * (BN / 2);
             const int row = m0 + quarter * 32 + lane;
             const bool valid = row < q.M;
-            const int c_first = colgrp * (bn / 2), c_end = c_first + bn / 2;
             uint32_t taddr;
 
-            if constexpr (EPI == kSum) {
+            // All columns of this warp (128, or 64 of a half-width tile) go to registers before anything is done with
+            // them: the loads overlap, and the accumulator goes back at once.
+            const int width = bn / 2, n_first = n0 + colgrp * width;
+            float v[128];
+            auto load_columns = [&]() {
                 const uint32_t acc = take(taddr);
-                if (!ok) break;
-                const float out_scale = q.out ? (p.count ? p.scale / fmaxf(*p.count, 1.f) : p.scale) : 1.f;
-                auto emit = [&](uint32_t* r, int c) {
-                    const int n = n0 + c;
-                    if (!valid || n >= q.N) return;
-                    const size_t at = (size_t)row * q.N + n;
-                    if (q.add) {
+                if (!ok) return;
 #pragma unroll
-                        for (int g = 0; g < 32; g += 8) {
-                            if (n + g >= q.N) break;       // N % 8 == 0: groups of eight are in or out together
+                for (int i = 0; i < 4; i++)
+                    if (i * 32 < width) tc::tmem_ld_32x32(taddr + colgrp * width + i * 32, (uint32_t*)v + i * 32);
+                tc::tmem_ld_wait();
+                pin(v);
+                give_back(acc);
+            };
+
+            if constexpr (EPI == kSum) {
+                load_columns();
+                if (!ok) break;
+                const int columns = min(width, q.N - n_first);       // N % 8 == 0: eight at a time are in or out
+                const size_t at = (size_t)row * q.N + n_first;
+                if (valid && q.add) {
+#pragma unroll
+                    for (int g = 0; g < 128; g += 8) {
+                        if (g < columns) {
                             float a[8];
                             load8_f32(a, q.add + at + g);
 #pragma unroll
-                            for (int j = 0; j < 8; j++) r[g + j] = __float_as_uint(__uint_as_float(r[g + j]) + a[j]);
+                            for (int j = 0; j < 8; j++) v[g + j] += a[j];
                         }
                     }
-                    store_sum<F16>(q, p.out_type, r, at, n, it.split, out_scale);
-                };
-                // a chunk is loaded from TMEM while the one before it is worked on
-                uint32_t ra[32], rb[32];
-                tc::tmem_ld_32x32(taddr + c_first, ra);
-#pragma unroll 1
-                for (int c = c_first; c < c_end; c += 64) {
-                    tc::tmem_ld_wait();
-                    tc::tmem_ld_32x32(taddr + c + 32, rb);
-                    emit(ra, c);
-                    tc::tmem_ld_wait();
-                    if (c + 64 < c_end) tc::tmem_ld_32x32(taddr + c + 64, ra);
-                    emit(rb, c + 32);
                 }
-                give_back(acc);
+                if (valid && q.out == nullptr)
+                    store_f32(q.sum + (size_t)it.split * q.M * q.N + at, v, columns, 1.f, true);
+                else if (valid) {
+                    const float scale = p.count ? p.scale / fmaxf(*p.count, 1.f) : p.scale;
+                    if (p.out_type == NVQ_F32) store_f32((float*)q.out + at, v, columns, scale, q.vec32);
+                    else store_16<F16>((uint16_t*)q.out + at, v, columns, scale, q.vec32);
+                }
             } else {
                 // Two bias buffers, by the tile's parity: the barrier in take() lies between the last reads of one
                 // and its next writes.
@@ -464,28 +462,17 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                         label -= p.v0;
                     }
                 }
-                const int width = bn / 2;                 // columns of this warp: 128, or 64 of a half-width tile
-                const int n_first = n0 + c_first;
-                float v[128];
-                // All columns of this warp lie in registers before anything is done with them: the loads overlap, the
-                // accumulator goes back at once, and maximum and sum run over 128 independent values.
-                uint32_t acc = take(taddr);
+                load_columns();
                 if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i * 32 < width) tc::tmem_ld_32x32(taddr + c_first + i * 32, (uint32_t*)v + i * 32);
-                tc::tmem_ld_wait();
-                pin(v);
-                give_back(acc);
                 if constexpr (EPI == kLse) {
                     for (int k0 = PART_KB; k0 < it.kb1; k0 += PART_KB) {
-                        acc = take(taddr);
+                        const uint32_t acc = take(taddr);
                         if (!ok) break;
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             if (i * 16 >= width) continue;
                             float r[16];
-                            tc::tmem_ld_32x16(taddr + c_first + i * 16, (uint32_t*)r);
+                            tc::tmem_ld_32x16(taddr + colgrp * width + i * 16, (uint32_t*)r);
                             tc::tmem_ld_wait();
                             pin(r);
 #pragma unroll
@@ -501,7 +488,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
 #pragma unroll
                     for (int j = 0; j < 128; j += 8) {
                         float b8[8];
-                        load8_f32(b8, bi + c_first + j);
+                        load8_f32(b8, bi + colgrp * width + j);
 #pragma unroll
                         for (int k = 0; k < 8; k += 2)
                             unpair2(add2(pair2(v[j + k], v[j + k + 1]), pair2(b8[k], b8[k + 1])), v[j + k], v[j + k + 1]);
@@ -802,6 +789,7 @@ nvq_status launch_after(void (*kernel)(KArgs...), size_t grid, int threads, int 
     return NVQ_OK;
 }
 
+int item_cost(int kb);
 template <int EPI, bool F16>
 nvq_status launch_gemm_typed(CeParams& p, const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
                        const CUtensorMap& b1, int device, cudaStream_t st) {
@@ -836,7 +824,7 @@ nvq_status launch_gemm_typed(CeParams& p, const CUtensorMap& a0, const CUtensorM
     if (p.q[1].num_items && p.q[0].num_items % used) {
         const int kb0 = p.q[0].splits > 1 ? p.q[0].kb_per : (p.q[0].K + BK - 1) / BK;
         const int kb1 = p.q[1].splits > 1 ? p.q[1].kb_per : (p.q[1].K + BK - 1) / BK;
-        p.lead = (kb0 + kb1 / 2) / kb1;
+        p.lead = (item_cost(kb0) + item_cost(kb1) / 2) / item_cost(kb1);
     }
     return launch_after(ce_gemm_kernel<EPI, F16>, 2 * (size_t)used, THREADS, SMEM_BYTES, st, a0, b0, a1, b1, p);
 }
@@ -851,13 +839,17 @@ size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 constexpr int kPairs = 74;      // what the splits are made for: workspace sizes are asked for without a device
 
-// The contractions of one launch as tiles and their length in k-blocks; splits[i] > 1: one item of a tile would take longer
-// than an even share of all work, and the tile is cut into parts of about that share, eight k-blocks at least.
+// The contractions of one launch as tiles and their length in k-blocks.  A tile takes as long as its MMAs or, with fewer than
+// EPILOGUE_KB k-blocks, as the writing of its result.  splits[i] > 1: one item of a tile would take longer than an
+// even share of all work, and the tile is cut into parts of about that share, eight k-blocks at least.
+constexpr int EPILOGUE_KB = 6;
+int item_cost(int kb) { return kb > EPILOGUE_KB ? kb : EPILOGUE_KB; }
 struct Shape { size_t M, N, K; };
 struct Cut { int splits, kb_per; };
 void cut_long(const Shape* q, Cut* cut, int n) {
     size_t total = 0;
-    for (int i = 0; i < n; i++) total += (q[i].M + BM - 1) / BM * ((q[i].N + BN - 1) / BN) * ((q[i].K + BK - 1) / BK);
+    for (int i = 0; i < n; i++)
+        total += (q[i].M + BM - 1) / BM * ((q[i].N + BN - 1) / BN) * item_cost((int)((q[i].K + BK - 1) / BK));
     size_t share = (total + kPairs - 1) / kPairs;
     if (share < 8) share = 8;
     for (int i = 0; i < n; i++) {
