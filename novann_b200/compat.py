@@ -42,7 +42,7 @@ def register_with_novann(novann=None) -> bool:
     for name in ("BatchNorm1d", "BatchNorm2d", "MaxPool2d", "GlobalAvgPool2d", "Flatten", "Dropout"):
         getattr(ref_layers, name).register(getattr(L, name))
     for cls in (L.Linear, L.Conv2d, L.ReLU, L.BatchNorm1d, L.BatchNorm2d, L.MaxPool2d,
-                L.GlobalAvgPool2d, L.Flatten, L.Dropout, Sequential):
+                L.GlobalAvgPool2d, L.Flatten, L.Dropout, L.Embedding, Sequential):
         RefLayer.register(cls)
     _registered = True
     return True

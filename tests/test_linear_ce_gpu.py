@@ -13,7 +13,7 @@ import pytest
 
 import novann_b200 as nb
 from novann_b200 import _lib, functional as F
-from novann_b200.device import DeviceBuffer, Stream, device_sync
+from novann_b200.device import DeviceBuffer, DeviceView, Stream, device_sync
 from oracle import oracle_np as o
 
 pytestmark = pytest.mark.gpu
@@ -265,6 +265,35 @@ def test_head_class_and_modes(gpu):
     assert head(x, y) == (loss, None)
     with pytest.raises(RuntimeError):
         head.backward()
+
+
+@pytest.mark.parametrize("dtype,grad", [("bf16", "bf16"), ("f16", "f32")])
+def test_buffers_on_16_byte_boundaries_and_nothing_behind_them(gpu, dtype, grad):
+    m, v, k = 130, 140, 64
+    size = 4 if grad == "f32" else 2
+    x, w, labels, _ = inputs(m, v, k, dtype, 11, bias=False)
+    r = reference(x, w, labels, None)
+    bx, bw = DeviceBuffer(x.nbytes + 16, gpu), DeviceBuffer(w.nbytes + 16, gpu)
+    bx.upload(x, offset=16)
+    bw.upload(w, offset=16)
+    bl = DeviceBuffer.from_numpy(labels.astype(np.int32), gpu)
+    ws = DeviceBuffer(F.linear_ce_workspace_bytes(m, v, k), gpu)
+    head, stats = DeviceBuffer(8, gpu), DeviceBuffer(m * 8, gpu)
+    view = lambda b: DeviceView(b.ptr + 16, b.nbytes - 16, gpu)  # noqa: E731
+    dx, dw = DeviceBuffer(16 + m * k * size + 16, gpu), DeviceBuffer(16 + v * k * size + 16, gpu)
+    for b in (dx, dw):
+        b.upload(np.full(b.nbytes, 0x5A, np.uint8))
+    F.linear_ce_device(head, stats, view(bx), view(bw), dtype, bl, m, v, k, ws)
+    F.linear_ce_bwd_device(view(dx), view(dw), view(bx), view(bw), dtype, bl, stats, head, m, v, k, ws, grad_dtype=grad)
+    device_sync(gpu)
+    F.check_device_errors(gpu)
+    t = {"f32": np.float32, "f16": np.float16, "bf16": np.uint16}[grad]
+    got = []
+    for b, n in ((dx, m), (dw, v)):
+        raw = b.to_numpy(np.uint8, (b.nbytes,))
+        assert np.all(raw[:16] == 0x5A) and np.all(raw[-16:] == 0x5A)
+        got.append(wide(raw[16:-16].view(t).reshape(n, k)))
+    check_grads(r, got[0], got[1], None, dtype, out=grad)
 
 
 def test_captured_graphs_share_a_workspace(gpu):
