@@ -148,6 +148,17 @@ struct SortParams {
     int* status;
 };
 
+// a warp writes n zeros, 32 bytes a lane between the boundaries
+__device__ __forceinline__ void clear_row(float* row, int n, int lane) {
+    const int head = min(n, (int)((32 - ((uintptr_t)row & 31)) & 31) / 4), octs = (n - head) / 8;
+    const u32x8 zero = {};
+    if (lane < head) row[lane] = 0.f;
+#pragma unroll 4
+    for (int i = lane; i < octs; i += 32) stg_stream_256(row + head + i * 8, zero);
+    const int tail = head + octs * 8 + lane;
+    if (tail < n) row[tail] = 0.f;
+}
+
 __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const SortParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     SortShared& sh = *(SortShared*)smem;
@@ -201,16 +212,9 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
             cluster_barrier();      // nobody reads this CTA's share any more
         }
         __syncthreads();
-        const bool wide = p.D % 8 == 0 && ((uintptr_t)p.clear & 31) == 0;
         for (size_t r = block * WARPS + warp; r < (size_t)p.vocab; r += blocks * WARPS) {      // a warp per row
             if (used[r >> 5] >> (r & 31) & 1u) continue;
-            float* row = p.clear + r * p.D;
-            if (wide)
-#pragma unroll 4
-                for (int c = lane * 8; c < p.D; c += 256) stg_stream_256(row + c, zero);
-            else
-#pragma unroll 4
-                for (int c = lane; c < p.D; c += 32) row[c] = 0.f;
+            clear_row(p.clear + r * p.D, p.D, lane);
         }
         return;
     }
@@ -554,6 +558,184 @@ join_runs_kernel(float* __restrict__ dtable, const float* __restrict__ carry, co
     }
 }
 
+// ---------------------------------------------------------------- few tokens: one launch, no sort
+// Up to FEW_TOKENS tokens, comparing every id with every other costs less than sorting: a warp per token looks for its
+// id among all T.  If an earlier token has it there is nothing to do; else the warp adds up the rows of all its
+// tokens, in order, and writes the table row.  An id with more than FEW_LIST tokens is left to the block, whose warps
+// then take a stretch of the tokens each.  The first blocks of the grid clear the rows that no token has.
+// Gradient of an 8191 x 1001 table: 64 tokens 8 us (sort, sums and join 19), 512 tokens 12 (19), 2048 tokens 30 (20):
+// the comparisons grow with T * T, and with them the time of an id that many tokens share.
+constexpr int FEW_WARPS = 8, FEW_LIST = 64, FEW_TOKENS = 512;
+constexpr size_t FEW_VOCAB = 262144;          // 32 KB of one bit per row
+
+template <int DT, int V>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 4)
+few_tokens_kernel(float* __restrict__ dtable, const void* __restrict__ dout, const int32_t* __restrict__ ids, int T,
+                  int vocab, int D, float scale, int padding_id, int accumulate, int clear_blocks, int groups,
+                  int tiles_per_group, int* __restrict__ status) {
+    using TL = Tile<DT, V>;
+    using E = Elem<DT>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int list[FEW_WARPS][FEW_LIST];
+    __shared__ int hot[FEW_WARPS];
+    __shared__ float part[FEW_WARPS][TL::COLS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if ((int)blockIdx.x < clear_blocks) {
+        uint32_t* used = (uint32_t*)smem;
+        for (int i = threadIdx.x; i < (vocab + 31) / 32; i += FEW_WARPS * 32) used[i] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (int i = threadIdx.x; i < T; i += FEW_WARPS * 32) {
+            const int id = ids[i];
+            if (id >= 0 && id < vocab && id != padding_id) atomicOr(&used[id >> 5], 1u << (id & 31));
+        }
+        __syncthreads();
+        for (int r = (int)blockIdx.x * FEW_WARPS + warp; r < vocab; r += clear_blocks * FEW_WARPS) {
+            if (used[r >> 5] >> (r & 31) & 1u) continue;
+            clear_row(dtable + (size_t)r * D, D, lane);
+        }
+        return;
+    }
+
+    const int block = (int)blockIdx.x - clear_blocks;
+    const int t = block / groups * FEW_WARPS + warp;
+    const int tile0 = block % groups * tiles_per_group;
+    const int tile1 = min(tile0 + tiles_per_group, (D + TL::COLS - 1) / TL::COLS);
+    const int id = t < T ? ids[t] : -1;
+    const bool inside = id >= 0 && id < vocab;
+    if (t < T && !inside && lane == 0 && status) atomicCAS(status, 0, ERR_ID_RANGE);
+    const char* base = (const char*)dout;
+    const size_t pitch = (size_t)D * E::SIZE;
+    // acc += the rows at[0 .. n) of one column tile
+    auto add_rows = [&](float* acc, const int* at, int n, int c0) {
+        constexpr int AHEAD = 4;
+        for (int j0 = 0; j0 < n; j0 += AHEAD) {
+            Packet<DT, V> q[AHEAD][TL::NV];
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+#pragma unroll
+                for (int k = 0; k < TL::NV; k++) {
+                    const int c = c0 + (k * 32 + lane) * V;
+                    if (j0 + a < n && c < D) q[a][k].load(base + (size_t)at[j0 + a] * pitch + (size_t)c * E::SIZE);
+                }
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+                if (j0 + a < n)
+#pragma unroll
+                    for (int k = 0; k < TL::NV; k++) {
+                        float f[V];
+                        q[a][k].widen(f);
+#pragma unroll
+                        for (int v = 0; v < V; v++) acc[k * V + v] += f[v];
+                    }
+        }
+    };
+
+    int n = 0;                  // tokens with this id, or FEW_LIST + 1 for more than the list holds
+    bool first = inside && id != padding_id;
+    for (int i0 = 0; i0 < T && first && n <= FEW_LIST; i0 += 8 * 32) {
+        int other[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int i = i0 + k * 32 + lane;
+            other[k] = i < T ? ids[i] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int i = i0 + k * 32 + lane;
+            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, other[k] == id);
+            if (hit == 0 || n > FEW_LIST) continue;
+            const int at = i0 + k * 32 + __ffs(hit) - 1;
+            if (at < t) {
+                first = false;
+                n = FEW_LIST + 1;       // ends the search
+                continue;
+            }
+            const int place = n + __popc(hit & ((1u << lane) - 1u));
+            if ((hit >> lane & 1u) && place < FEW_LIST) list[warp][place] = i;
+            n += __popc(hit);
+        }
+    }
+    __syncwarp();
+    if (first && n <= FEW_LIST)
+        for (int tile = tile0; tile < tile1; tile++) {
+            float acc[TL::E];
+#pragma unroll
+            for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
+            add_rows(acc, list[warp], n, tile * TL::COLS);
+            put_row<TL, V>(dtable + (size_t)id * D, acc, tile * TL::COLS, lane, D, scale, accumulate);
+        }
+    if (lane == 0) hot[warp] = first && n > FEW_LIST ? id : -1;
+    __syncthreads();
+    const int stretch = (T + FEW_WARPS * 32 - 1) / (FEW_WARPS * 32) * 32;      // tokens per warp, whole votes
+    for (int w = 0; w < FEW_WARPS; w++) {
+        const int id_w = hot[w];
+        if (id_w < 0) continue;
+        for (int tile = tile0; tile < tile1; tile++) {
+            float acc[TL::E];
+#pragma unroll
+            for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
+            int held = 0;
+            for (int i0 = warp * stretch; i0 < min(T, (warp + 1) * stretch); i0 += 32) {
+                const int i = i0 + lane;
+                const bool same = i < T && ids[i] == id_w;
+                const uint32_t hit = __ballot_sync(0xFFFFFFFFu, same);
+                if (same) list[warp][held + __popc(hit & ((1u << lane) - 1u))] = i;     // at most 31 + 32
+                held += __popc(hit);
+                __syncwarp();
+                if (held >= 32) {
+                    add_rows(acc, list[warp], held, tile * TL::COLS);
+                    held = 0;
+                    __syncwarp();
+                }
+            }
+            add_rows(acc, list[warp], held, tile * TL::COLS);
+#pragma unroll
+            for (int e = 0; e < TL::E; e++) part[warp][e * 32 + lane] = acc[e];
+            __syncthreads();
+            if (warp == w) {
+#pragma unroll
+                for (int e = 0; e < TL::E; e++) {
+                    acc[e] = part[0][e * 32 + lane];
+                    for (int x = 1; x < FEW_WARPS; x++) acc[e] += part[x][e * 32 + lane];
+                }
+                put_row<TL, V>(dtable + (size_t)id_w * D, acc, tile * TL::COLS, lane, D, scale, accumulate);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+template <int DT, int V>
+nvq_status few_tokens(float* dtable, const void* dout, const int32_t* ids, int T, int vocab, int D, float scale,
+                      int padding_id, int accumulate, int* status, int device, cudaStream_t st) {
+    const int sms = nvq_sm_count(device), blocks = (T + FEW_WARPS - 1) / FEW_WARPS;
+    const int tiles = (D + Tile<DT, V>::COLS - 1) / Tile<DT, V>::COLS;
+    // column tiles go to more blocks until there are about 24 a SM
+    int groups = (24 * sms + blocks - 1) / blocks;
+    if (groups > tiles) groups = tiles;
+    const int per_group = (tiles + groups - 1) / groups;
+    groups = (tiles + per_group - 1) / per_group;
+    const size_t bytes = accumulate ? 0 : ((size_t)vocab + 31) / 32 * 4;
+    size_t clear = accumulate ? 0 : ((size_t)vocab * D + 8191) / 8192;
+    if (clear > (size_t)2 * sms) clear = 2 * sms;
+    few_tokens_kernel<DT, V><<<(unsigned)(clear + (size_t)blocks * groups), FEW_WARPS * 32, bytes, st>>>(
+        dtable, dout, ids, T, vocab, D, scale, padding_id, accumulate, (int)clear, groups, per_group, status);
+    NVQ_LAUNCHED();
+    return NVQ_OK;
+}
+
+template <int DT>
+nvq_status few_tokens_of(float* dtable, const void* dout, const int32_t* ids, int T, int vocab, int D, float scale,
+                         int padding_id, int accumulate, int* status, int device, cudaStream_t st) {
+    constexpr int V16 = 16 / Elem<DT>::SIZE, V4 = 4 / Elem<DT>::SIZE;
+    if (D % V16 == 0 && nvq_aligned(dout, 16) && nvq_aligned(dtable, 16))
+        return few_tokens<DT, V16>(dtable, dout, ids, T, vocab, D, scale, padding_id, accumulate, status, device, st);
+    if (V4 > 1 && D % V4 == 0 && nvq_aligned(dout, 4))
+        return few_tokens<DT, V4>(dtable, dout, ids, T, vocab, D, scale, padding_id, accumulate, status, device, st);
+    return few_tokens<DT, 1>(dtable, dout, ids, T, vocab, D, scale, padding_id, accumulate, status, device, st);
+}
+
 cudaLaunchConfig_t sort_launch(size_t grid, int cluster, cudaStream_t st, cudaLaunchAttribute* attr) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
@@ -686,6 +868,14 @@ extern "C" nvq_status nvq_embedding_bwd(float* d_dtable, const void* d_dout, nvq
     int* status = nullptr;
     s = nvq_status_word(device, &status);
     if (s != NVQ_OK) return s;
+    if (T <= (size_t)FEW_TOKENS && (accumulate || V <= FEW_VOCAB)) {
+        const int t = (int)T, v = (int)V, d = (int)D;
+        if (dout_dtype == NVQ_F32)
+            return few_tokens_of<NVQ_F32>(d_dtable, d_dout, d_ids, t, v, d, scale, padding_id, accumulate, status, device, st);
+        if (dout_dtype == NVQ_F16)
+            return few_tokens_of<NVQ_F16>(d_dtable, d_dout, d_ids, t, v, d, scale, padding_id, accumulate, status, device, st);
+        return few_tokens_of<NVQ_BF16>(d_dtable, d_dout, d_ids, t, v, d, scale, padding_id, accumulate, status, device, st);
+    }
     static std::atomic<int> clusters[64];    // per device: sorting clusters that run at once (found twice: harmless)
     if (!clusters[device]) {
         NVQ_CUDA(cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
