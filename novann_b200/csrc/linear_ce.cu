@@ -25,8 +25,6 @@ constexpr int BM = 256, BN = 256, BK = 64, UMMA_K = 16;
 constexpr int A_BYTES = 128 * BK * 2, B_BYTES = 128 * BK * 2;   // per CTA
 constexpr int STAGES = 6;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 8192;
 constexpr int TMEM_COLS = 512;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -34,6 +32,15 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float F16_GAIN = 16384.f;
 
 enum { kLse = 0, kProb = 1, kSum = 2 };
+// Epilogue warps: eight with 128 columns of 32 rows each, in registers (168 a thread).  kProb, which has the most to do
+// per column, is faster with sixteen of 64 columns (2048 x 32000 x 1024: 115 us against 124), the others are not (kLse
+// 107 against 102).
+template <int EPI> struct Cfg {
+    static constexpr int WARPS = EPI == kProb ? 16 : 8;
+    static constexpr int THREADS = 64 + 32 * WARPS;
+    static constexpr int COLGRPS = WARPS / 4, COLS = BN / COLGRPS;
+};
+constexpr int MAX_WARPS = 16, LSE_SLOTS = Cfg<kLse>::COLGRPS;      // partial maxima and sums per 256 columns
 enum { ERR_PRODUCER = 81, ERR_MMA_FULL = 82, ERR_MMA_TMEM = 83, ERR_EPILOGUE = 84, ERR_LABEL = 85 };
 
 // One contraction: (M x K) times (K x N) in 256 x 256 tiles
@@ -53,7 +60,7 @@ struct CeParams {
     // kLse, kProb
     const float* bias;
     const int32_t* labels;
-    float2* partial;             // kLse: (2 * n_blocks) x M maxima and sums
+    float2* partial;             // kLse: (LSE_SLOTS * n_blocks) x M maxima and sums
     float* label_logit;          // kLse: M
     const float* stats;          // kProb: M row maxima, then M logarithms of the sums of exp(l - maximum)
     int v0, vocab, ignore;       // kProb: first vocabulary entry of this piece, vocabulary, label that does not count
@@ -77,7 +84,7 @@ struct Shared {
     uint32_t tmem_base;
     int abort_flag;
     alignas(16) float bias[2][BN];
-    float db_part[EPI_WARPS][32];
+    float db_part[MAX_WARPS][32];
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -177,9 +184,10 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
 }
 
 // `columns` of one row's sums, times s; wide: dst lies on a 32-byte boundary, else on a 16-byte one
-__device__ __forceinline__ void store_f32(float* dst, const float (&v)[128], int columns, float s, bool wide) {
+template <int COLS>
+__device__ __forceinline__ void store_f32(float* dst, const float (&v)[COLS], int columns, float s, bool wide) {
 #pragma unroll
-    for (int g = 0; g < 128; g += 8) {
+    for (int g = 0; g < COLS; g += 8) {
         if (g >= columns) break;
         u32x8 o;
 #pragma unroll
@@ -192,10 +200,10 @@ __device__ __forceinline__ void store_f32(float* dst, const float (&v)[128], int
         }
     }
 }
-template <bool F16>
-__device__ __forceinline__ void store_16(uint16_t* dst, const float (&v)[128], int columns, float s, bool wide) {
+template <bool F16, int COLS>
+__device__ __forceinline__ void store_16(uint16_t* dst, const float (&v)[COLS], int columns, float s, bool wide) {
 #pragma unroll
-    for (int g = 0; g < 128; g += 16) {
+    for (int g = 0; g < COLS; g += 16) {
         if (g >= columns) break;
         u32x8 o;
 #pragma unroll
@@ -212,11 +220,12 @@ __device__ __forceinline__ void store_16(uint16_t* dst, const float (&v)[128], i
 // kLse, kProb: both operands with the contraction contiguous.  kSum: B with N contiguous, A as Problem::a_mn says.
 // F16: operands (and 16-bit results) are fp16, else bf16.
 template <int EPI, bool F16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1)
 ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
                const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
                const __grid_constant__ CeParams p) {
     constexpr bool B_MN = EPI == kSum;
+    constexpr int EPI_WARPS = Cfg<EPI>::WARPS, COLGRPS = Cfg<EPI>::COLGRPS, COLS = Cfg<EPI>::COLS;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = tc::smem_u32(smem_raw);
     const uint32_t tiles = (raw + 1023u) & ~1023u;
@@ -347,8 +356,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
     } else {
         // ------------------------------------------------------------ epilogue (both CTAs)
         const int quarter = warp & 3;                 // the TMEM lanes this warp may read
-        const int colgrp = (warp - 2) >> 2;           // which 128 (64) columns of the tile
-        const int et = threadIdx.x - 64;              // 0 .. 255
+        const int colgrp = (warp - 2) >> 2;           // which COLS (COLS / 2) columns of the tile
+        const int et = threadIdx.x - 64;
         bool ok = true;
         int n_acc = 0;
         // the accumulator that comes next, complete; every epilogue thread takes part, whatever its lane found
@@ -405,15 +414,15 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
             const bool valid = row < q.M;
             uint32_t taddr;
 
-            // All columns of this warp (128, or 64 of a half-width tile) go to registers before anything is done with
-            // them: the loads overlap, and the accumulator goes back at once.
-            const int width = bn / 2, n_first = n0 + colgrp * width;
-            float v[128];
+            // All columns of this warp (COLS, or half as many of a half-width tile) go to registers before anything is
+            // done with them: the loads overlap, and the accumulator goes back at once.
+            const int width = bn / COLGRPS, n_first = n0 + colgrp * width;
+            float v[COLS];
             auto load_columns = [&]() {
                 const uint32_t acc = take(taddr);
                 if (!ok) return;
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < COLS / 32; i++)
                     if (i * 32 < width) tc::tmem_ld_32x32(taddr + colgrp * width + i * 32, (uint32_t*)v + i * 32);
                 tc::tmem_ld_wait();
                 pin(v);
@@ -427,7 +436,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                 const size_t at = (size_t)row * q.N + n_first;
                 if (valid && q.add) {
 #pragma unroll
-                    for (int g = 0; g < 128; g += 8) {
+                    for (int g = 0; g < COLS; g += 8) {
                         if (g < columns) {
                             float a[8];
                             load8_f32(a, q.add + at + g);
@@ -469,7 +478,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                         const uint32_t acc = take(taddr);
                         if (!ok) break;
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
+                        for (int i = 0; i < COLS / 16; i++) {
                             if (i * 16 >= width) continue;
                             float r[16];
                             tc::tmem_ld_32x16(taddr + colgrp * width + i * 16, (uint32_t*)r);
@@ -486,7 +495,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                 }
                 if (p.bias) {
 #pragma unroll
-                    for (int j = 0; j < 128; j += 8) {
+                    for (int j = 0; j < COLS; j += 8) {
                         float b8[8];
                         load8_f32(b8, bi + colgrp * width + j);
 #pragma unroll
@@ -495,9 +504,9 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                     }
                 }
                 const int columns = min(width, q.N - n_first);     // the rest lies past the vocabulary
-                if (columns < 128) {
+                if (columns < COLS) {
 #pragma unroll
-                    for (int j = 0; j < 128; j++)
+                    for (int j = 0; j < COLS; j++)
                         if (j >= columns) v[j] = -INFINITY;
                 }
                 const int hit = label - n_first;          // the label's place among this warp's columns
@@ -505,19 +514,19 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                 if constexpr (EPI == kLse) {
                     if (hit >= 0 && hit < columns) {
 #pragma unroll
-                        for (int j = 0; j < 128; j++)
+                        for (int j = 0; j < COLS; j++)
                             if (j == hit) p.label_logit[row] = v[j];
                     }
                     float m[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++) m[j] = v[j];
 #pragma unroll
-                    for (int j = 4; j < 124; j += 8) {
+                    for (int j = 4; j < COLS - 4; j += 8) {
 #pragma unroll
                         for (int k = 0; k < 4; k++) m[k] = max3(m[k], v[j + 2 * k], v[j + 2 * k + 1]);
                     }
                     const float top = max3(max3(m[0], m[1], m[2]), m[3],
-                                           max3(fmaxf(v[124], v[125]), v[126], v[127]));
+                                           max3(fmaxf(v[COLS - 4], v[COLS - 3]), v[COLS - 2], v[COLS - 1]));
                     // exp(l - top) by one multiply-add, off by 2^-24 of |top| in the exponent, as the logits are
                     float s1 = -top * LOG2E;
                     if (!__all_sync(0xFFFFFFFFu, fabsf(top) < 1e30f)) {
@@ -525,13 +534,13 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                         // row whose entries are all taken out has sum 0 relative to 0.
                         const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                        for (int j = 0; j < 128; j++) v[j] -= ref;
+                        for (int j = 0; j < COLS; j++) v[j] -= ref;
                         s1 = 0.f;
                     }
                     const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(s1, s1);
                     uint64_t s2[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int j = 0; j < 128; j += 2) {
+                    for (int j = 0; j < COLS; j += 2) {
                         float a, b;
                         unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
                         s2[j / 2 % 4] = add2(s2[j / 2 % 4], pair2(ex2(a), ex2(b)));
@@ -541,19 +550,19 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                     // the maximum and sum of this warp's columns, for each of its rows (kLse tiles are never cut in
                     // two, so a 256-column block has these two entries)
                     if (valid)
-                        p.partial[(size_t)(it.tile.n_blk * 2 + colgrp) * q.M + row] = make_float2(top, s_even + s_odd);
+                        p.partial[(size_t)(it.tile.n_blk * COLGRPS + colgrp) * q.M + row] = make_float2(top, s_even + s_odd);
                 } else {
                     // softmax(l) - onehot, times F16_GAIN (2^14, part of the exponent) for fp16
                     constexpr float gain = F16 ? F16_GAIN : 1.f, log2_gain = F16 ? 14.f : 0.f;
                     float s1 = log2_gain - (row_max * LOG2E + log2_sum);      // off by 2^-15 of a probability at most
                     if (!__all_sync(0xFFFFFFFFu, fabsf(row_max) < 256.f)) {
 #pragma unroll
-                        for (int j = 0; j < 128; j++) v[j] -= row_max;
+                        for (int j = 0; j < COLS; j++) v[j] -= row_max;
                         s1 = log2_gain - log2_sum;
                     }
                     const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(s1, s1);
 #pragma unroll
-                    for (int j = 0; j < 128; j += 2) {
+                    for (int j = 0; j < COLS; j += 2) {
                         float a, b;
                         unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
                         v[j] = ex2(a);
@@ -561,7 +570,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                     }
                     if (hit >= 0 && hit < columns) {
 #pragma unroll
-                        for (int j = 0; j < 128; j++)
+                        for (int j = 0; j < COLS; j++)
                             if (j == hit) v[j] -= gain;
                     }
                     // a row that does not count gives zeros whatever its logits are
@@ -569,7 +578,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                     if (valid) {
                         uint16_t* dst = p.prob + (size_t)row * p.ldp + n_first;
 #pragma unroll
-                        for (int g = 0; g < 128; g += 16) {
+                        for (int g = 0; g < COLS; g += 16) {
                             if (g < width && n_first + g < p.ldp) {
                                 u32x8 o;
 #pragma unroll
@@ -584,7 +593,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                         // columns that its lane bit names and adds its partner's; after five steps lane l holds
                         // column l.
 #pragma unroll
-                        for (int c = 0; c < 128; c += 32) {
+                        for (int c = 0; c < COLS; c += 32) {
                             if (c >= width) continue;
                             float f[32];
 #pragma unroll
@@ -826,7 +835,7 @@ nvq_status launch_gemm_typed(CeParams& p, const CUtensorMap& a0, const CUtensorM
         const int kb1 = p.q[1].splits > 1 ? p.q[1].kb_per : (p.q[1].K + BK - 1) / BK;
         p.lead = (item_cost(kb0) + item_cost(kb1) / 2) / item_cost(kb1);
     }
-    return launch_after(ce_gemm_kernel<EPI, F16>, 2 * (size_t)used, THREADS, SMEM_BYTES, st, a0, b0, a1, b1, p);
+    return launch_after(ce_gemm_kernel<EPI, F16>, 2 * (size_t)used, Cfg<EPI>::THREADS, SMEM_BYTES, st, a0, b0, a1, b1, p);
 }
 template <int EPI>
 nvq_status launch_gemm(CeParams& p, bool f16, const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
@@ -875,7 +884,7 @@ size_t piece_of(size_t M, size_t V) {
 struct FwdSpace { size_t partial, logit, block, total; };
 FwdSpace fwd_space(size_t M, size_t V) {
     FwdSpace s;
-    s.partial = align256((V + BN - 1) / BN * 2 * M * sizeof(float2));
+    s.partial = align256((V + BN - 1) / BN * LSE_SLOTS * M * sizeof(float2));
     s.logit = align256(M * 4);
     s.block = align256((M + 31) / 32 * sizeof(double2));
     s.total = s.partial + s.logit + s.block;
@@ -997,7 +1006,7 @@ extern "C" nvq_status nvq_linear_ce_fwd(float* d_loss_count, float* d_row_loss, 
     s = launch_gemm<kLse>(p, dtype == NVQ_F16, a, b, a, b, device, st);
     if (s != NVQ_OK) return s;
     // up to eight partial sums a row: a warp adds up 32 rows by itself; more: the whole block does
-    const int slots = 2 * p.q[0].n_blocks, mean = reduction == NVQ_REDUCE_MEAN;
+    const int slots = LSE_SLOTS * p.q[0].n_blocks, mean = reduction == NVQ_REDUCE_MEAN;
     const int rows = slots <= 8 ? 32 * JOIN_WARPS : 32, blocks = (int)((M + rows - 1) / rows);
     s = slots <= 8 ? launch_after(join_rows_kernel<1>, blocks, JOIN_WARPS * 32, 0, st, d_loss_count, d_row_stats,
                                   d_row_loss, block_sum, partial, logit, d_labels, (int)M, slots, (int)V, ignore_index,
