@@ -1,6 +1,6 @@
 """novann_b200: B200-native (sm_100a) casts, FP8 / FP4 quantisation, quantised Linear / Conv2d
-and the fp32 layers of NovaNN's CNN for NovaNN's NumPy-array API, over the C ABI in
-``include/nvq.h``.
+the fp32 layers of NovaNN's CNN and the operators of token models (embedding, linear cross
+entropy, gradient clipping) for NovaNN's NumPy-array API, over the C ABI in ``include/nvq.h``.
 
 No layer arithmetic runs on the CPU: every operation calls ``libnvq.so`` and fails loudly if
 the library or a GPU is missing.  (``Dropout`` draws its keep mask from NumPy's generator on
