@@ -1,4 +1,4 @@
-"""novann_b200: B200-native (sm_100a) casts, FP8 / FP4 quantisation, quantised Linear / Conv2d
+"""novann_b200: B200-native (sm_100a) casts, FP8 / FP4 quantisation, quantised Linear / Conv2d,
 the fp32 layers of NovaNN's CNN and the operators of token models (embedding, linear cross
 entropy, gradient clipping) for NovaNN's NumPy-array API, over the C ABI in ``include/nvq.h``.
 
