@@ -10,7 +10,8 @@
 // contiguous (the contraction for X W^T and for g in dX; the other one for W in dX and for both
 // operands of dW - the tensor core reads either, so nothing is ever transposed) and the epilogue:
 //   kLse   per row the maximum and the sum of exp over 128 columns, and the label's logit
-//   kProb  softmax(l) - onehot as 16-bit values, a piece of the vocabulary at a time
+//   kProb  softmax(l) - onehot as 16-bit values, a piece of the vocabulary at a time (kProbDb: and the
+//          column sums of the fp32 values, for db)
 //   kSum   fp32 sums: added to a buffer, or scaled and rounded to the gradient's type
 // The backward pass computes the logits of a piece a second time instead of keeping M x V of them:
 // 8 M V K operations where 6 M V K are needed, against reading and writing the logits twice.
@@ -27,16 +28,17 @@ constexpr int STAGES = 6;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 8192;
 constexpr int TMEM_COLS = 512;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // fp16 values of g below 2^-14 would lose bits: they are kept times 2^14 (|g| <= 1 stays in range)
 constexpr float F16_GAIN = 16384.f;
 
-enum { kLse = 0, kProb = 1, kSum = 2 };
+enum { kLse = 0, kProb = 1, kSum = 2, kProbDb = 3 };
+constexpr bool is_prob(int epi) { return epi == kProb || epi == kProbDb; }
 // Epilogue warps: eight with 128 columns of 32 rows each, in registers (168 a thread).  kProb, which has the most to do
-// per column, is faster with sixteen of 64 columns (2048 x 32000 x 1024: 115 us against 124), the others are not (kLse
+// per column, is faster with sixteen of 64 columns (2048 x 32000 x 1024: 114 us against 124), the others are not (kLse
 // 107 against 102).
 template <int EPI> struct Cfg {
-    static constexpr int WARPS = EPI == kProb ? 16 : 8;
+    static constexpr int WARPS = is_prob(EPI) ? 16 : 8;
     static constexpr int THREADS = 64 + 32 * WARPS;
     static constexpr int COLGRPS = WARPS / 4, COLS = BN / COLGRPS;
 };
@@ -66,7 +68,7 @@ struct CeParams {
     int v0, vocab, ignore;       // kProb: first vocabulary entry of this piece, vocabulary, label that does not count
     uint16_t* prob;              // kProb: M x ldp, ldp a multiple of 16, 0 past the piece
     int ldp;
-    float* col_partial;          // ceil(M / 32) x ldp column sums of 32 rows each (kProb writes, kSum adds up), or nullptr
+    float* col_partial;          // ceil(M / 32) x ldp column sums of 32 rows each (kProbDb writes, kSum adds up)
     // kSum
     int out_type;
     float scale;                 // factor of the final results, over the count of rows where `count` is set
@@ -97,6 +99,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+// a + b, and in `lost` exactly what its rounding left out (Knuth's two-sum)
+__device__ __forceinline__ float two_sum(float a, float b, float& lost) {
+    const float s = __fadd_rn(a, b), t = __fsub_rn(s, a);
+    lost = __fadd_rn(__fsub_rn(a, __fsub_rn(s, t)), __fsub_rn(b, t));
+    return s;
 }
 // two fp32 operations in one instruction
 __device__ __forceinline__ uint64_t pair2(float a, float b) {
@@ -172,11 +180,14 @@ __device__ __forceinline__ int nth_item(const CeParams& p, int pair, int num_pai
     return i < n1 ? n0 + i : -1;
 }
 
-// kLse keeps at most this many k-blocks (1024 of K) in one TMEM accumulator: the tensor core cuts off where it adds, by
-// up to a step of the running sum each time, and over 4096 of K the logits were off by 1e-6 of themselves, all
-// towards zero.  The parts are joined in registers; MMAs and epilogue alternate between the two accumulators as
-// they do between tiles.
-constexpr int PART_KB = 16;
+// kLse and kProbDb keep at most this many k-blocks (512 of K) in one TMEM accumulator: the tensor core cuts off where it
+// adds, by up to a step of the running sum each time.  Over 4096 of K the logits were off by 1e-6 of themselves, all
+// towards zero; in parts of 1024 the row losses are 6e-7 off, in parts of 512 3e-7 (and scoring 4095 x 50001 x 2048
+// takes 517 us instead of 506).  The parts are joined in registers; MMAs and epilogue alternate between the two
+// accumulators as they do between tiles.  db needs the probabilities from logits summed alike: from one
+// accumulator they missed a sum of 1 by 3e-5 at K = 4096.
+constexpr int PART_KB = 8;
+constexpr bool in_parts(int epi) { return epi == kLse || epi == kProbDb; }
 
 template <bool F16>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
@@ -217,6 +228,14 @@ __device__ __forceinline__ void store_16(uint16_t* dst, const float (&v)[COLS], 
     }
 }
 
+// 32 lanes x 8 consecutive fp32 columns
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, float* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
 // kLse, kProb: both operands with the contraction contiguous.  kSum: B with N contiguous, A as Problem::a_mn says.
 // F16: operands (and 16-bit results) are fp16, else bf16.
 template <int EPI, bool F16>
@@ -236,7 +255,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
     volatile int* abort_flag = &sh->abort_flag;
     // accumulators: two of 256 columns
     auto acc_of = [&](int n, uint32_t& acc, uint32_t& acc_phase) { acc = n & 1; acc_phase = (n >> 1) & 1; };
-    const int part_kb = EPI == kLse ? PART_KB : 1 << 30;
+    constexpr int part_kb = in_parts(EPI) ? PART_KB : 1 << 30;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -459,13 +478,13 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                 for (int c = et; c < bn; c += 32 * EPI_WARPS)
                     bi[c] = p.bias && n0 + c < q.N ? p.bias[n0 + c] : 0.f;
                 int label = -1;              // column of this launch, or out of its range
-                [[maybe_unused]] float row_max = 0.f, log2_sum = 0.f;
+                [[maybe_unused]] float row_max = 0.f, log_sum = 0.f;
                 [[maybe_unused]] bool counts = false;
                 if (valid) {
                     label = p.labels[row];
-                    if constexpr (EPI == kProb) {
+                    if constexpr (is_prob(EPI)) {
                         row_max = p.stats[row];
-                        log2_sum = p.stats[(size_t)q.M + row] * LOG2E;
+                        log_sum = p.stats[(size_t)q.M + row];
                         // a row whose every entry is taken out (-inf) has no gradient
                         counts = label != p.ignore && label >= 0 && label < p.vocab && row_max != -INFINITY;
                         label -= p.v0;
@@ -473,21 +492,23 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                 }
                 load_columns();
                 if (!ok) break;
-                if constexpr (EPI == kLse) {
+                if constexpr (in_parts(EPI)) {
+                    constexpr int W = EPI == kLse ? 16 : 8;      // columns at a time: what the registers leave room for
                     for (int k0 = PART_KB; k0 < it.kb1; k0 += PART_KB) {
                         const uint32_t acc = take(taddr);
                         if (!ok) break;
 #pragma unroll
-                        for (int i = 0; i < COLS / 16; i++) {
-                            if (i * 16 >= width) continue;
-                            float r[16];
-                            tc::tmem_ld_32x16(taddr + colgrp * width + i * 16, (uint32_t*)r);
+                        for (int i = 0; i < COLS / W; i++) {
+                            if (i * W >= width) continue;
+                            float r[W];
+                            if constexpr (W == 16) tc::tmem_ld_32x16(taddr + colgrp * width + i * W, (uint32_t*)r);
+                            else tmem_ld_32x8(taddr + colgrp * width + i * W, r);
                             tc::tmem_ld_wait();
                             pin(r);
 #pragma unroll
-                            for (int j = 0; j < 16; j += 2)
-                                unpair2(add2(pair2(v[i * 16 + j], v[i * 16 + j + 1]), pair2(r[j], r[j + 1])), v[i * 16 + j],
-                                        v[i * 16 + j + 1]);
+                            for (int j = 0; j < W; j += 2)
+                                unpair2(add2(pair2(v[i * W + j], v[i * W + j + 1]), pair2(r[j], r[j + 1])), v[i * W + j],
+                                        v[i * W + j + 1]);
                         }
                         give_back(acc);
                     }
@@ -527,7 +548,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                     }
                     const float top = max3(max3(m[0], m[1], m[2]), m[3],
                                            max3(fmaxf(v[COLS - 4], v[COLS - 3]), v[COLS - 2], v[COLS - 1]));
-                    // exp(l - top) by one multiply-add, off by 2^-24 of |top| in the exponent, as the logits are
+                    // exp(l - top) by one multiply-add
                     float s1 = -top * LOG2E;
                     if (!__all_sync(0xFFFFFFFFu, fabsf(top) < 1e30f)) {
                         // Logits near the lowest fp32 value, whose product with log2 e overflows, or nothing but -inf: a
@@ -547,24 +568,35 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                     }
                     float s_even, s_odd;
                     unpair2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), s_even, s_odd);
+                    float sum = s_even + s_odd;
+                    // what the shift lost in rounding, as a factor 2^e = 1 + e ln 2 of all of them
+                    if (s1 != 0.f) sum = fmaf(sum * fmaf(-top, LOG2E, -s1), LN2, sum);
                     // the maximum and sum of this warp's columns, for each of its rows (kLse tiles are never cut in
                     // two, so a 256-column block has these two entries)
                     if (valid)
-                        p.partial[(size_t)(it.tile.n_blk * COLGRPS + colgrp) * q.M + row] = make_float2(top, s_even + s_odd);
+                        p.partial[(size_t)(it.tile.n_blk * COLGRPS + colgrp) * q.M + row] = make_float2(top, sum);
                 } else {
                     // softmax(l) - onehot, times F16_GAIN (2^14, part of the exponent) for fp16
                     constexpr float gain = F16 ? F16_GAIN : 1.f, log2_gain = F16 ? 14.f : 0.f;
-                    float s1 = log2_gain - (row_max * LOG2E + log2_sum);      // off by 2^-15 of a probability at most
+                    // by one multiply-add, whose shift is off by 2^-15 of a probability at most; kProbDb adds what it lost
+                    const float a_hi = row_max * LOG2E, b_hi = log_sum * LOG2E;
+                    const float b_lo = fmaf(log_sum, LOG2E, -b_hi);
+                    float lost, left;
+                    float s1 = two_sum(log2_gain, -two_sum(a_hi, b_hi, lost), left);
+                    [[maybe_unused]] float s0 = left - (lost + fmaf(row_max, LOG2E, -a_hi) + b_lo);
                     if (!__all_sync(0xFFFFFFFFu, fabsf(row_max) < 256.f)) {
 #pragma unroll
                         for (int j = 0; j < COLS; j++) v[j] -= row_max;
-                        s1 = log2_gain - log2_sum;
+                        s1 = log2_gain - b_hi;
+                        s0 = -b_lo;
                     }
                     const uint64_t scale = pair2(LOG2E, LOG2E), shift = pair2(s1, s1);
 #pragma unroll
                     for (int j = 0; j < COLS; j += 2) {
+                        uint64_t t = fma2(pair2(v[j], v[j + 1]), scale, shift);
+                        if constexpr (EPI == kProbDb) t = add2(t, pair2(s0, s0));
                         float a, b;
-                        unpair2(fma2(pair2(v[j], v[j + 1]), scale, shift), a, b);
+                        unpair2(t, a, b);
                         v[j] = ex2(a);
                         v[j + 1] = ex2(b);
                     }
@@ -588,7 +620,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
                             }
                         }
                     }
-                    if (p.col_partial) {
+                    if constexpr (EPI == kProbDb) {
                         // Sums of 32 columns over the warp's 32 rows: at each step a lane keeps the half of its
                         // columns that its lane bit names and adds its partner's; after five steps lane l holds
                         // column l.
@@ -1081,7 +1113,8 @@ extern "C" nvq_status nvq_linear_ce_bwd(void* d_dx, void* d_dw, nvq_dtype grad_d
         p.prob = prob;
         p.ldp = (int)ld;
         p.col_partial = d_db ? cols : nullptr;
-        s = launch_gemm<kProb>(p, f16, x_k, w_k, x_k, w_k, device, st);
+        s = d_db ? launch_gemm<kProbDb>(p, f16, x_k, w_k, x_k, w_k, device, st)
+                 : launch_gemm<kProb>(p, f16, x_k, w_k, x_k, w_k, device, st);
         if (s != NVQ_OK) return s;
 
         // dX and dW of the piece in one launch, and db beside them

@@ -211,6 +211,16 @@ def test_large_and_equal_logits(gpu):
     assert np.all(np.abs(row[labels >= 0] - np.log(v)) <= 8 * 2.0 ** -22)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_probabilities_of_a_row_sum_to_one(gpu, dtype):
+    """Both passes sum a logit alike, so the gradients of the biases sum to 0 up to what follows the logits: exp2 and
+    its argument's rounding (2^-21 of each probability) and fp32 sums over the entries and rows, however long K is."""
+    m, v, k = 300, 41, 4096
+    x, w, labels, b = inputs(m, v, k, dtype, 12)
+    db = F.linear_ce_host(x, w, labels, b, device=gpu)[4].astype(np.float64)
+    assert abs(db.sum()) <= 2.0 ** -21 + v * 2.0 ** -24 + m * 2.0 ** -24 * np.abs(db).sum()
+
+
 def test_labels_out_of_range_are_reported(gpu):
     x, w, labels, _ = inputs(4, 20, 16, "bf16", 8, ignore=False)
     labels[1], labels[2] = 20, -1
