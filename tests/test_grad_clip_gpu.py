@@ -68,7 +68,7 @@ def check(arrays, dtypes, max_norm, head, got):
 
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16", "f64"])
-@pytest.mark.parametrize("counts", [[1], [4095], [4096], [4097], [1, 2, 3, 70000], [0, 5, 0], [12345] * 5])
+@pytest.mark.parametrize("counts", [[1], [4095], [4096], [4097], [8191, 8192, 8193], [16384, 16385], [1, 2, 3, 70000], [0, 5, 0], [12345] * 5])
 def test_clip_one_type(gpu, in_place, dtype, counts):
     rng = np.random.default_rng(sum(counts))
     arrays = [to_type(rng.standard_normal(n), dtype) for n in counts]
