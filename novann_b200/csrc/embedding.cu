@@ -159,6 +159,40 @@ __device__ __forceinline__ void clear_row(float* row, int n, int lane) {
     if (tail < n) row[tail] = 0.f;
 }
 
+// this block's share of the whole table
+__device__ __forceinline__ void clear_flat(const SortParams& p, size_t block, size_t blocks, int threads) {
+    const size_t floats = (size_t)p.vocab * p.D;
+    const size_t first = block * threads + threadIdx.x, step = blocks * threads;
+    const size_t octs = ((uintptr_t)p.clear & 31) == 0 ? floats / 8 : 0;
+    const u32x8 zero = {};
+#pragma unroll 4
+    for (size_t i = first; i < octs; i += step) stg_stream_256(p.clear + 8 * i, zero);
+    for (size_t i = octs * 8 + first; i < floats; i += step) p.clear[i] = 0.f;
+}
+// this warp's share of the rows whose bit is not set
+__device__ __forceinline__ void clear_unused(const SortParams& p, const uint32_t* used, size_t warp, size_t warps,
+                                             int lane) {
+    for (size_t r = warp; r < (size_t)p.vocab; r += warps)
+        if (!(used[r >> 5] >> (r & 31) & 1u)) clear_row(p.clear + r * p.D, p.D, lane);
+}
+// the sets of the bits of this thread's ids, every `step`-th from `first`
+__device__ __forceinline__ void mark_used(const SortParams& p, uint32_t* used, int first, int step) {
+    for (int i0 = first; i0 < p.n; i0 += 8 * step) {
+        int id[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int i = i0 + k * step;
+            id[k] = i < p.n ? p.ids[i] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (id[k] >= 0 && id[k] < p.vocab && id[k] != p.padding_id) {
+                const uint32_t bit = 1u << (id[k] & 31);
+                if (!(*(volatile uint32_t*)&used[id[k] >> 5] & bit)) atomicOr(&used[id[k] >> 5], bit);
+            }
+    }
+}
+
 __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const SortParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     SortShared& sh = *(SortShared*)smem;
@@ -169,14 +203,8 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
 
     if (blockIdx.x >= ctas) {               // not the sorting cluster: clear the table
         const size_t block = blockIdx.x - ctas, blocks = gridDim.x - ctas;
-        const u32x8 zero = {};
         if (!p.skip_used) {
-            const size_t floats = (size_t)p.vocab * p.D;
-            const size_t first = block * SORT_THREADS + tid, step = blocks * SORT_THREADS;
-            const size_t octs = ((uintptr_t)p.clear & 31) == 0 ? floats / 8 : 0;
-#pragma unroll 4
-            for (size_t i = first; i < octs; i += step) stg_stream_256(p.clear + 8 * i, zero);
-            for (size_t i = octs * 8 + first; i < floats; i += step) p.clear[i] = 0.f;
+            clear_flat(p, block, blocks, SORT_THREADS);
             return;
         }
         // One bit per row: each CTA of the cluster looks at its share of the ids, then the shares are joined.
@@ -184,20 +212,8 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
         uint32_t *share = (uint32_t*)smem, *used = share + (ctas > 1 ? words : 0);
         for (int i = tid; i < words; i += SORT_THREADS) share[i] = 0;
         __syncthreads();
-        for (int i0 = (int)rank * SORT_THREADS + tid; i0 < p.n; i0 += 8 * (int)ctas * SORT_THREADS) {
-            int id[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int i = i0 + k * (int)ctas * SORT_THREADS;
-                id[k] = i < p.n ? p.ids[i] : -1;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (id[k] >= 0 && id[k] < p.vocab && id[k] != p.padding_id) {
-                    const uint32_t bit = 1u << (id[k] & 31);
-                    if (!(*(volatile uint32_t*)&share[id[k] >> 5] & bit)) atomicOr(&share[id[k] >> 5], bit);
-                }
-        }
+        mark_used(p, share, (int)rank * SORT_THREADS + tid, (int)ctas * SORT_THREADS);
+        __syncthreads();
         if (ctas > 1) {
             cluster_barrier();
             for (int i = tid; i < words; i += SORT_THREADS) {
@@ -212,10 +228,7 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
             cluster_barrier();      // nobody reads this CTA's share any more
         }
         __syncthreads();
-        for (size_t r = block * WARPS + warp; r < (size_t)p.vocab; r += blocks * WARPS) {      // a warp per row
-            if (used[r >> 5] >> (r & 31) & 1u) continue;
-            clear_row(p.clear + r * p.D, p.D, lane);
-        }
+        clear_unused(p, used, block * WARPS + warp, blocks * WARPS, lane);
         return;
     }
 
@@ -359,7 +372,11 @@ constexpr int PIECE = 32;
 constexpr int SUM_WARPS = 4;
 
 template <int DT, int V> struct Tile {
-    static constexpr int NV = (16 / Elem<DT>::SIZE) / V;      // packets per lane: 16 bytes in all
+    // Packets per lane: one of 16 bytes, or narrow ones of 8 bytes in all and twice as many rows under way (65536 rows of
+    // 1001 bf16: 60 us against 70 with 16 bytes; two rows of one wide packet more: 79 us against 70)
+    static constexpr bool NARROW = V * Elem<DT>::SIZE < 16;
+    static constexpr int NV = NARROW ? (8 / Elem<DT>::SIZE) / V : 1;
+    static constexpr int AHEAD = NARROW ? 16 : 8;
     static constexpr int E = V * NV;
     static constexpr int COLS = 32 * E;
 };
@@ -422,7 +439,7 @@ sum_runs_kernel(float* __restrict__ dtable, float* __restrict__ carry, const voi
 #pragma unroll
     for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
     bool head = __shfl_sync(0xFFFFFFFFu, id, 0) == prev;      // the first run began in an earlier piece
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = TL::AHEAD;
     for (int j0 = 0; j0 < live; j0 += AHEAD) {
         Packet<DT, V> q[AHEAD][TL::NV];
 #pragma unroll
@@ -911,7 +928,7 @@ extern "C" nvq_status nvq_embedding_bwd(float* d_dtable, const void* d_dout, nvq
         // tokens are all there are: later parts add to rows that have to be 0).
         q.skip_used = D >= 1024 && V <= sizeof(SortShared) * 4 - 64 && T <= (size_t)SORT_MAX;
         q.status = status;
-        const int ctas = n <= SORT_THREADS ? 1 : MAX_CLUSTER;
+        const int ctas = n <= SORT_THREADS ? 1 : MAX_CLUSTER;      // the last part of many may be short
         q.chunk_log2 = 5;
         while (((size_t)ctas << q.chunk_log2) < (size_t)n) q.chunk_log2++;
         // Further clusters clear the table: as many as run beside the sorting one (128 of 148 SMs take clusters of eight;

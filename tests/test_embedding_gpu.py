@@ -88,7 +88,7 @@ def test_ids_out_of_range_are_reported_and_give_zeros(gpu):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("t,v,d", [(1, 1, 1), (1, 9, 5), (31, 3, 64), (32, 1, 8), (33, 1, 8), (64, 2, 12), (1000, 7, 40),
-                                   (1024, 600, 33), (512, 3, 100), (513, 3, 100), (512, 300000, 7), (500, 400, 261), (1025, 511, 130), (4095, 512, 260), (20000, 70000, 4),
+                                   (1024, 600, 33), (512, 3, 100), (513, 3, 100), (512, 300000, 7), (500, 400, 261), (1025, 511, 130), (4095, 512, 260), (4096, 200000, 9), (4097, 3, 30), (2000, 130, 1025), (20000, 70000, 4),
                                    (5000, 300, 1001), (131072, 1000, 2), (131073, 5, 3)])
 def test_table_gradient(gpu, dtype, t, v, d):
     rng = np.random.default_rng(t * 7 + d)
@@ -102,7 +102,7 @@ def test_table_gradient(gpu, dtype, t, v, d):
     assert np.array_equal(got.view(np.uint32), again.view(np.uint32))
 
 
-@pytest.mark.parametrize("t", [500, 10000])
+@pytest.mark.parametrize("t", [500, 3000, 10000])
 @pytest.mark.parametrize("case", ["one id", "sorted", "all padding", "last id"])
 def test_table_gradient_extremes(gpu, case, t):
     v, d = 257, 72
