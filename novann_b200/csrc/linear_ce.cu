@@ -95,6 +95,12 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
+// Waits for the kernel before this one; the kernel after it may then be set up beside this one (it waits alike).
+__device__ __forceinline__ void chain() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -284,7 +290,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant
     tc::cluster_sync_all();
     tc::tc_fence_after();
     const uint32_t tmem_base = sh->tmem_base;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    chain();
 
     if (warp == 0) {
         // ------------------------------------------------------------ producer (both CTAs)
@@ -688,7 +694,7 @@ join_rows_kernel(float* __restrict__ loss_out, float* __restrict__ stats, float*
     __shared__ double sums[JOIN_WARPS], counts[JOIN_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = (blockIdx.x * (JOIN_WARPS / WAYS) + warp / WAYS) * 32 + lane;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    chain();
     float m = -INFINITY, s = 0.f;
     if (row < M) {
         int i = warp % WAYS;
@@ -746,7 +752,7 @@ join_rows_kernel(float* __restrict__ loss_out, float* __restrict__ stats, float*
 __global__ void __launch_bounds__(256)
 loss_kernel(float* __restrict__ loss_out, const double2* __restrict__ block_sum, int blocks, int mean) {
     __shared__ double sums[8], counts[8];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    chain();
     double s = 0.0, n = 0.0;
     for (int i = threadIdx.x; i < blocks; i += 256) {
         s += block_sum[i].x;
@@ -770,7 +776,7 @@ template <int DT>
 __global__ void __launch_bounds__(256)
 join_splits_kernel(void* out, const float* __restrict__ parts, int splits, const float* add, size_t n,
                    float scale, const float* __restrict__ count) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    chain();
     const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     float f[4] = {0.f, 0.f, 0.f, 0.f};
@@ -799,7 +805,7 @@ bias_grad_kernel(float* __restrict__ db, const float* __restrict__ col_partial, 
     __shared__ float part[8][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.x * 32 + lane;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    chain();
     float s = 0.f;
     if (c < N)
 #pragma unroll 4
