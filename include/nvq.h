@@ -385,7 +385,7 @@ nvq_status nvq_embedding_fwd(void* d_out, const void* d_table, nvq_dtype dtype, 
  * bits on every call); accumulate != 0 adds to what d_dtable holds (a table that is also the output
  * projection: its gradient from there first), otherwise rows without a token become 0.  Tokens whose id
  * is padding_id take no part (a negative padding_id: none is padding); ids outside [0, V) take no part and
- * are reported (code 71).  D <= 2^22.  Workspace: nvq_embedding_bwd_workspace_bytes, 256-byte aligned,
+ * are reported (code 71).  D <= 2^21.  Workspace: nvq_embedding_bwd_workspace_bytes, 256-byte aligned,
  * contents need not be kept or cleared between calls.  More than 131072 tokens run as parts of that
  * many, one after the other. */
 nvq_status nvq_embedding_bwd_workspace_bytes(size_t T, size_t V, size_t D, size_t* bytes);

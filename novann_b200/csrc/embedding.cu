@@ -866,8 +866,8 @@ extern "C" nvq_status nvq_embedding_bwd(float* d_dtable, const void* d_dout, nvq
                                         int device, void* stream) {
     NVQ_REQUIRE(dout_dtype == NVQ_F32 || dout_dtype == NVQ_F16 || dout_dtype == NVQ_BF16,
                 "nvq_embedding_bwd: gradient type %d; f32, f16 and bf16 are taken", (int)dout_dtype);
-    NVQ_REQUIRE(V > 0 && V < (1u << 31) - 1 && D > 0 && D <= (1u << 22) && T < ((size_t)1 << 31),
-                "nvq_embedding_bwd: V in [1, 2^31 - 1), D in [1, 2^22], T below 2^31");
+    NVQ_REQUIRE(V > 0 && V < (1u << 31) - 1 && D > 0 && D <= (1u << 21) && T < ((size_t)1 << 31),
+                "nvq_embedding_bwd: V in [1, 2^31 - 1), D in [1, 2^21], T below 2^31");
     const size_t size = dout_dtype == NVQ_F32 ? 4 : 2;
     NVQ_REQUIRE(d_dtable && nvq_aligned(d_dtable, 4), "nvq_embedding_bwd: null or misaligned table gradient");
     NVQ_REQUIRE(T == 0 || (d_dout && d_ids && nvq_aligned(d_dout, size) && nvq_aligned(d_ids, 4)),

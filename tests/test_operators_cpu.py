@@ -36,6 +36,7 @@ def test_embedding_refusals():
     refused(g(ODD, P, _lib.F32, P, 100, 10, 8, 1.0, -1, 0, P, need, 0, None), "table gradient")
     refused(g(P, None, _lib.F32, P, 100, 10, 8, 1.0, -1, 0, P, need, 0, None), "null")
     refused(g(P, P, _lib.F32, P, 100, 10, (1 << 22) + 1, 1.0, -1, 0, P, 1 << 62, 0, None), "D in")
+    refused(g(P, P, _lib.F32, P, 100, 10, (1 << 21) + 1, 1.0, -1, 0, P, 1 << 62, 0, None), "D in")
 
 
 def test_embedding_host_refusals():
