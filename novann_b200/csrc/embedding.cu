@@ -420,6 +420,7 @@ sum_runs_kernel(float* __restrict__ dtable, float* __restrict__ carry, const voi
     const int lane = threadIdx.x & 31;
     const int piece = blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the next one waits alike
     if (piece >= pieces) return;
     const int c0 = blockIdx.y * TL::COLS;
     const int i0 = piece * PIECE;

@@ -118,6 +118,7 @@ __device__ __forceinline__ double chunk_squares_f64(const double* p, int n) {
 template <int NT>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM)
 square_sum_kernel(const __grid_constant__ TensorList<NT> L, double* __restrict__ partial, uint32_t chunks, int add) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the next kernel is set up, and waits
     __shared__ double sh[THREADS / 32];
     double s = 0.0;
     int t = 0;
