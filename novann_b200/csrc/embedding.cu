@@ -365,11 +365,13 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_tokens_kernel(const Sort
 
 // ---------------------------------------------------------------- sums over runs of one id
 // A warp adds the rows of PIECE consecutive sorted tokens over a tile of columns.  A run of one id
-// that lies inside the piece goes straight to the table; the two that may cross its ends leave
-// partial sums in `carry` (slot 0: a run that began in an earlier piece, slot 1: one that begins here
-// and goes on), which join_runs_kernel adds up in the order of the pieces.
+// that lies inside the piece goes straight to the table; the two that may cross its ends are joined in shared
+// memory over the pieces of the block, in their order.  The two that may cross the block's ends leave partial
+// sums in `carry` (slot 0: a run that began in an earlier block, slot 1: one that begins here and goes
+// on), which join_runs_kernel adds up in the order of the blocks.
 constexpr int PIECE = 32;
 constexpr int SUM_WARPS = 4;
+constexpr int BLOCK_TOKENS = PIECE * SUM_WARPS;
 
 template <int DT, int V> struct Tile {
     // Packets per lane: one of 16 bytes, or narrow ones of 8 bytes in all and twice as many rows under way (65536 rows of
@@ -411,26 +413,28 @@ __device__ __forceinline__ void put_row(float* row, const float* acc, int c0, in
 }
 
 template <int DT, int V>
-__global__ void __launch_bounds__(SUM_WARPS * 32)
+__global__ void __launch_bounds__(SUM_WARPS * 32, 5)       // 96 registers: narrow packets would take 128
 sum_runs_kernel(float* __restrict__ dtable, float* __restrict__ carry, const void* __restrict__ dout,
                 const int32_t* __restrict__ sorted_id, const int32_t* __restrict__ sorted_pos, int n, int vocab, int D,
-                int pieces, float scale, int accumulate) {
+                float scale, int accumulate) {
     using TL = Tile<DT, V>;
     using E = Elem<DT>;
-    const int lane = threadIdx.x & 31;
-    const int piece = blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
+    // the sums of a piece's first run, if it began earlier, and of its last, if it goes on; HEAD_TAIL: they are one
+    enum { HEAD = 1, TAIL = 2, HEAD_TAIL = 4 };
+    __shared__ float head_sum[SUM_WARPS][TL::COLS], tail_sum[SUM_WARPS][TL::COLS];
+    __shared__ int kinds[SUM_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int piece = blockIdx.x * SUM_WARPS + warp;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the next one waits alike
-    if (piece >= pieces) return;
     const int c0 = blockIdx.y * TL::COLS;
-    const int i0 = piece * PIECE;
+    const int i0 = piece * PIECE;          // past the last token: a piece without any
     const int my = i0 + lane;
     const int id = my < n ? sorted_id[my] : vocab;
     const int pos = my < n ? sorted_pos[my] : 0;
-    const int prev = i0 > 0 ? sorted_id[i0 - 1] : -1;
+    const int prev = i0 > 0 && i0 < n ? sorted_id[i0 - 1] : -1;
     const int next = i0 + PIECE < n ? sorted_id[i0 + PIECE] : vocab;
     const int live = __popc(__ballot_sync(0xFFFFFFFFu, id < vocab));     // the tokens that count come first
-    if (live == 0) return;
     // bit j: the run that item j belongs to ends with it, inside this piece
     const int right = __shfl_down_sync(0xFFFFFFFFu, id, 1);
     const uint32_t ends = __ballot_sync(0xFFFFFFFFu, lane == PIECE - 1 || right != id);
@@ -440,6 +444,7 @@ sum_runs_kernel(float* __restrict__ dtable, float* __restrict__ carry, const voi
 #pragma unroll
     for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
     bool head = __shfl_sync(0xFFFFFFFFu, id, 0) == prev;      // the first run began in an earlier piece
+    int kind = 0, tail_id = 0;
     constexpr int AHEAD = TL::AHEAD;
     for (int j0 = 0; j0 < live; j0 += AHEAD) {
         Packet<DT, V> q[AHEAD][TL::NV];
@@ -467,25 +472,59 @@ sum_runs_kernel(float* __restrict__ dtable, float* __restrict__ carry, const voi
             if ((ends >> j) & 1u) {
                 const int run = __shfl_sync(0xFFFFFFFFu, id, j);
                 const bool tail = j == PIECE - 1 && run == next;
-                if (head || tail)
-                    put_row<TL, V>(carry + ((size_t)piece * 2 + (head ? 0 : 1)) * D, acc, c0, lane, D, 1.f, false);
-                else
+                if (head || tail) {
+                    float* keep = head ? head_sum[warp] : tail_sum[warp];
+#pragma unroll
+                    for (int e = 0; e < TL::E; e++) keep[e * 32 + lane] = acc[e];
+                    kind |= head ? (tail ? HEAD | HEAD_TAIL : HEAD) : TAIL;
+                    tail_id = run;
+                } else {
                     put_row<TL, V>(dtable + (size_t)run * D, acc, c0, lane, D, scale, accumulate);
+                }
                 head = false;
 #pragma unroll
                 for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
             }
         }
     }
+    if (lane == 0) kinds[warp] = kind;
+    __syncthreads();
+    auto add = [&](const float* from) {
+#pragma unroll
+        for (int e = 0; e < TL::E; e++) acc[e] += from[e * 32 + lane];
+    };
+    float* out = carry + (size_t)blockIdx.x * 2 * D;
+    if (kind & TAIL) {
+#pragma unroll
+        for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
+        add(tail_sum[warp]);
+        bool on = true;             // the run goes on behind this block
+        for (int w = warp + 1; w < SUM_WARPS && on; w++) {
+            add(head_sum[w]);
+            on = kinds[w] & HEAD_TAIL;
+        }
+        if (on) put_row<TL, V>(out + D, acc, c0, lane, D, 1.f, false);
+        else put_row<TL, V>(dtable + (size_t)tail_id * D, acc, c0, lane, D, scale, accumulate);
+    }
+    if (warp == 0 && (kind & HEAD)) {
+#pragma unroll
+        for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
+        bool on = true;
+        for (int w = 0; w < SUM_WARPS && on; w++) {
+            add(head_sum[w]);
+            on = kinds[w] & HEAD_TAIL;
+        }
+        put_row<TL, V>(out, acc, c0, lane, D, 1.f, false);
+    }
 }
 
-// The runs that cross pieces: slot 1 of the piece where one begins, then slot 0 of every piece that it
-// reaches.  A warp looks at one piece and adds up a run of at most LONG_RUN pieces by itself; a longer one
-// (a frequent token: one in sixteen tokens of a 65536-token batch makes 128 pieces) is cut into equal
-// parts for the warps of the block, whose sums are then added in order.
+// The runs that cross those blocks: slot 1 of the block where one begins, then slot 0 of every block that it
+// reaches.  A warp looks at one of them and adds up a run of at most LONG_RUN by itself; a longer one
+// (a frequent token: one in sixteen tokens of a 65536-token batch makes 32 blocks) is cut into equal
+// shares for the warps, whose sums are then added in order.
 constexpr int JOIN_WARPS = 8, LONG_RUN = 16;
 
-// 256 columns a warp and four blocks an SM: most blocks see within three loads that no run begins in their pieces, and
+// 256 columns a warp and four blocks an SM: most blocks see within three loads that no run begins in their parts, and
 // the few that have something to add up should all be there at once.
 template <int V> struct JoinTile {
     static constexpr int NV = 8 / V, E = 8, COLS = 256;
@@ -494,10 +533,10 @@ template <int V> struct JoinTile {
 template <int V>
 __global__ void __launch_bounds__(JOIN_WARPS * 32, 4)
 join_runs_kernel(float* __restrict__ dtable, const float* __restrict__ carry, const int32_t* __restrict__ sorted_id,
-                 int n, int vocab, int D, int pieces, float scale, int accumulate) {
+                 int n, int vocab, int D, int parts, float scale, int accumulate) {
     using TL = JoinTile<V>;
-    __shared__ int run_pieces[JOIN_WARPS];      // pieces after the first, for the block to add up; 0: none
-    __shared__ float part[JOIN_WARPS][TL::COLS];
+    __shared__ int run_parts[JOIN_WARPS];      // parts after the first, for the block to add up; 0: none
+    __shared__ float share[JOIN_WARPS][TL::COLS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c0 = blockIdx.y * TL::COLS;
     auto fetch = [&](const float* row, float* f) {
@@ -511,7 +550,7 @@ join_runs_kernel(float* __restrict__ dtable, const float* __restrict__ carry, co
             q.widen(f + k * V);
         }
     };
-    auto add_slots = [&](float* acc, int first, int many) {       // slot 0 of `many` pieces from `first`
+    auto add_slots = [&](float* acc, int first, int many) {       // slot 0 of `many` parts from `first`
         constexpr int AHEAD = 4;
         for (int a0 = 0; a0 < many; a0 += AHEAD) {
             float f[AHEAD][TL::E];
@@ -526,18 +565,18 @@ join_runs_kernel(float* __restrict__ dtable, const float* __restrict__ carry, co
         }
     };
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int piece0 = blockIdx.x * JOIN_WARPS;
-    const int piece = piece0 + warp;
+    const int part0 = blockIdx.x * JOIN_WARPS;
+    const int part = part0 + warp;
     int many = 0, id = vocab;
-    if (piece + 1 < pieces) {
-        const int i0 = piece * PIECE, i1 = i0 + PIECE;      // i1 < n: another piece follows
+    if (part + 1 < parts) {
+        const int i0 = part * BLOCK_TOKENS, i1 = i0 + BLOCK_TOKENS;      // i1 < n: another part follows
         id = sorted_id[i1 - 1];
         const bool begins = id < vocab && sorted_id[i1] == id &&
                             !(sorted_id[i0] == id && i0 > 0 && sorted_id[i0 - 1] == id);
-        // a piece belongs to the run while its first token has the run's id
-        for (int q0 = piece + 1; begins && q0 < pieces; q0 += 32) {
+        // a part belongs to the run while its first token has the run's id
+        for (int q0 = part + 1; begins && q0 < parts; q0 += 32) {
             const int mine = q0 + lane;
-            const bool in = mine < pieces && sorted_id[(size_t)mine * PIECE] == id;
+            const bool in = mine < parts && sorted_id[(size_t)mine * BLOCK_TOKENS] == id;
             const uint32_t hit = __ballot_sync(0xFFFFFFFFu, in);
             many += hit == 0xFFFFFFFFu ? 32 : __ffs(~hit) - 1;
             if (hit != 0xFFFFFFFFu) break;
@@ -545,30 +584,30 @@ join_runs_kernel(float* __restrict__ dtable, const float* __restrict__ carry, co
     }
     if (many > 0 && many <= LONG_RUN) {
         float acc[TL::E];
-        fetch(carry + ((size_t)piece * 2 + 1) * D, acc);
-        add_slots(acc, piece + 1, many);
+        fetch(carry + ((size_t)part * 2 + 1) * D, acc);
+        add_slots(acc, part + 1, many);
         put_row<TL, V>(dtable + (size_t)id * D, acc, c0, lane, D, scale, accumulate);
     }
-    if (lane == 0) run_pieces[warp] = many > LONG_RUN ? many : 0;
+    if (lane == 0) run_parts[warp] = many > LONG_RUN ? many : 0;
     __syncthreads();
     for (int w = 0; w < JOIN_WARPS; w++) {
-        const int total = run_pieces[w];
+        const int total = run_parts[w];
         if (total == 0) continue;
         const int each = (total + JOIN_WARPS - 1) / JOIN_WARPS;
         const int first = warp * each, mine = max(0, min(each, total - first));
         float acc[TL::E];
 #pragma unroll
         for (int e = 0; e < TL::E; e++) acc[e] = 0.f;
-        if (warp == 0) fetch(carry + ((size_t)(piece0 + w) * 2 + 1) * D, acc);
-        add_slots(acc, piece0 + w + 1 + first, mine);
+        if (warp == 0) fetch(carry + ((size_t)(part0 + w) * 2 + 1) * D, acc);
+        add_slots(acc, part0 + w + 1 + first, mine);
 #pragma unroll
-        for (int e = 0; e < TL::E; e++) part[warp][e * 32 + lane] = acc[e];
+        for (int e = 0; e < TL::E; e++) share[warp][e * 32 + lane] = acc[e];
         __syncthreads();
         if (warp == w) {
 #pragma unroll
             for (int e = 0; e < TL::E; e++) {
-                acc[e] = part[0][e * 32 + lane];
-                for (int x = 1; x < JOIN_WARPS; x++) acc[e] += part[x][e * 32 + lane];
+                acc[e] = share[0][e * 32 + lane];
+                for (int x = 1; x < JOIN_WARPS; x++) acc[e] += share[x][e * 32 + lane];
             }
             put_row<TL, V>(dtable + (size_t)id * D, acc, c0, lane, D, scale, accumulate);
         }
@@ -777,7 +816,7 @@ BwdSpace bwd_space(size_t T, size_t D) {
     BwdSpace s;
     s.ids = align256(n * 4);
     s.pos = align256(n * 4);
-    s.carry = align256((n + PIECE - 1) / PIECE * 2 * D * 4);
+    s.carry = align256((n + BLOCK_TOKENS - 1) / BLOCK_TOKENS * 2 * D * 4);
     s.total = s.ids + s.pos + s.carry;
     return s;
 }
@@ -801,30 +840,28 @@ template <int DT>
 nvq_status sum_runs(float* dtable, float* carry, const char* dout, const int32_t* sid, const int32_t* spos, int n,
                     int vocab, int D, float scale, int accumulate, cudaStream_t st) {
     constexpr int V16 = 16 / Elem<DT>::SIZE, V4 = 4 / Elem<DT>::SIZE;
-    const int pieces = (n + PIECE - 1) / PIECE;
+    const int parts = (n + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
     const bool wide = D % V16 == 0 && nvq_aligned(dout, 16) && nvq_aligned(dtable, 16);
     const dim3 block(SUM_WARPS * 32);
-    auto grid = [&](int cols, int warps = SUM_WARPS) {
-        return dim3((pieces + warps - 1) / warps, (D + cols - 1) / cols);
-    };
+    auto grid = [&](int cols, int each = 1) { return dim3((parts + each - 1) / each, (D + cols - 1) / cols); };
     const int join = JOIN_WARPS * 32;
     if (wide)
         launch_after(sum_runs_kernel<DT, V16>, grid(Tile<DT, V16>::COLS), block, st, dtable, carry, dout, sid, spos, n,
-                     vocab, D, pieces, scale, accumulate);
+                     vocab, D, scale, accumulate);
     else if (V4 > 1 && D % V4 == 0 && nvq_aligned(dout, 4))
         launch_after(sum_runs_kernel<DT, V4>, grid(Tile<DT, V4>::COLS), block, st, dtable, carry, dout, sid, spos, n,
-                     vocab, D, pieces, scale, accumulate);
+                     vocab, D, scale, accumulate);
     else
         launch_after(sum_runs_kernel<DT, 1>, grid(Tile<DT, 1>::COLS), block, st, dtable, carry, dout, sid, spos, n, vocab,
-                     D, pieces, scale, accumulate);
+                     D, scale, accumulate);
     NVQ_LAUNCHED();
-    if (pieces > 1) {
+    if (parts > 1) {
         if (D % 4 == 0 && nvq_aligned(dtable, 16))
             launch_after(join_runs_kernel<4>, grid(JoinTile<4>::COLS, JOIN_WARPS), join, st, dtable, carry, sid, n, vocab,
-                         D, pieces, scale, accumulate);
+                         D, parts, scale, accumulate);
         else
             launch_after(join_runs_kernel<1>, grid(JoinTile<1>::COLS, JOIN_WARPS), join, st, dtable, carry, sid, n, vocab,
-                         D, pieces, scale, accumulate);
+                         D, parts, scale, accumulate);
         NVQ_LAUNCHED();
     }
     return NVQ_OK;

@@ -116,6 +116,20 @@ def test_table_gradient_extremes(gpu, case, t):
     assert np.all(np.abs(got - want) <= tol)
 
 
+@pytest.mark.parametrize("d", [3, 72, 261])
+@pytest.mark.parametrize("first", [0, 31])
+def test_runs_of_every_length_from_every_place(gpu, first, d):
+    """Ids with 1, 2, ... 300 tokens: runs of the sorted tokens that begin and end anywhere, and some that cover whole
+    blocks of them."""
+    lengths = np.concatenate([np.ones(first, int), np.arange(1, 301)])
+    rng = np.random.default_rng(first + d)
+    ids = rng.permutation(np.repeat(np.arange(len(lengths)), lengths)).astype(np.int32)
+    dout = rng.standard_normal((ids.size, d)).astype(np.float32)
+    got = F.embedding_bwd_host(dout, ids, len(lengths) + 2, device=gpu)
+    want, tol = want_grad(dout, ids, len(lengths) + 2, 1.0, None)
+    assert np.all(np.abs(got - want) <= tol)
+
+
 def test_padding_rows_may_hold_anything_and_infinities_stay_in_their_row(gpu):
     dout = np.ones((6, 16), np.float32)
     ids = np.array([0, 3, 1, 3, 2, 1], np.int32)
