@@ -381,7 +381,7 @@ nvq_status nvq_adamw_step_f32(float* d_param, const float* d_grad, float* d_m, f
  * of zeros and is reported by nvq_device_error_flag (code 71). */
 nvq_status nvq_embedding_fwd(void* d_out, const void* d_table, nvq_dtype dtype, const int32_t* d_ids,
                              size_t T, size_t V, size_t D, float scale, int device, void* stream);
-/* d_dtable (V x D fp32) = scale * sum of d_dout's rows per id, added in fp32 in the order of t (the same
+/* d_dtable (V x D fp32) = scale * sum of d_dout's rows per id, added in fp32 in a fixed order (the same
  * bits on every call); accumulate != 0 adds to what d_dtable holds (a table that is also the output
  * projection: its gradient from there first), otherwise rows without a token become 0.  Tokens whose id
  * is padding_id take no part (a negative padding_id: none is padding); ids outside [0, V) take no part and

@@ -1,6 +1,6 @@
 // Embedding lookup, out[t] = scale * table[id_t], and the gradient of its table,
 //   dtable[v] = scale * sum over t with id_t == v of dout[t]        (+ dtable[v] when accumulating)
-// added for every v in the order of t, in fp32, without atomics: equal inputs give equal bits.
+// added for every v in a fixed order, in fp32, without atomics: equal inputs give equal bits.
 #include "packet.cuh"
 
 nvq_status nvq_status_word(int device, int** dev_ptr);
