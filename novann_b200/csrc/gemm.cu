@@ -255,7 +255,12 @@ nvq_status nvq_status_word(int device, int** dev_ptr) {
     std::lock_guard<std::mutex> lock(g_status_mu);
     if (!g_status_host[device]) {
         int* h = nullptr;
-        NVQ_CUDA(cudaHostAlloc((void**)&h, sizeof(int), cudaHostAllocMapped));
+        // the first call of a process may be one that is being captured: the allocation is not part of the graph
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        NVQ_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t e = cudaHostAlloc((void**)&h, sizeof(int), cudaHostAllocMapped);
+        NVQ_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        NVQ_CUDA(e);
         *h = 0;
         NVQ_CUDA(cudaHostGetDevicePointer((void**)&g_status_dev[device], h, 0));
         g_status_host[device] = h;

@@ -5,6 +5,9 @@ The bounds follow the gradients': a value of g is off by the operands' half step
 roundings by n * 2^-23 of the magnitudes that were added; the norm is off by at most the norm of all errors.
 """
 import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -195,3 +198,44 @@ def test_offsets_past_32_bits(gpu):
     assert np.all(np.abs(dx[-last:] - g @ ws_) <= tol)
     tol = H * (np.abs(g).T @ np.abs(xs)) + 2.0 ** -12 * (p / last).T @ np.abs(xs)
     assert np.all(np.abs(dw - g.T @ xs) <= tol)
+
+
+FIRST_CALLS = """
+import ctypes as C
+import numpy as np
+from novann_b200 import _lib, functional as F
+from novann_b200.device import DeviceBuffer, Stream
+gpu, (t, v, d) = int({gpu}), (1000, 300, 64)
+rng = np.random.default_rng(0)
+ids = DeviceBuffer.from_numpy(rng.integers(0, v, t).astype(np.int32), gpu)
+table = DeviceBuffer.from_numpy(rng.standard_normal((v, d)).astype(np.float16), gpu)
+out, dx, dw, dtable = (DeviceBuffer(n, gpu) for n in (t * d * 2, t * d * 4, v * d * 4, v * d * 4))
+loss, stats, norm = DeviceBuffer(8, gpu), DeviceBuffer(t * 8, gpu), DeviceBuffer(8, gpu)
+ws = DeviceBuffer(max(F.embedding_bwd_workspace_bytes(t, v, d), F.linear_ce_workspace_bytes(t, v, d),
+                      F.grad_norm_workspace_bytes()), gpu)
+st = Stream(gpu)
+def step():
+    F.embedding_device(out, table, "f16", ids, t, v, d, stream=st)
+    F.linear_ce_device(loss, stats, out, table, "f16", ids, t, v, d, ws, stream=st)
+    F.linear_ce_bwd_device(dx, dw, out, table, "f16", ids, stats, loss, t, v, d, ws, stream=st)
+    F.embedding_bwd_device(dtable, dx, "f32", ids, t, v, d, ws, stream=st)
+    F.clip_grads_device(norm, [dw, dtable], [v * d] * 2, "f32", 1e-3, ws, stream=st)
+def results():
+    st.sync()
+    return [b.to_numpy(np.uint32, (b.nbytes // 4,)) for b in (out, loss, dw, dtable, norm)]
+exe = C.c_void_p()
+_lib.check(_lib.lib().nvq_graph_begin_capture(gpu, C.c_void_p(st.ptr)))
+step()
+_lib.check(_lib.lib().nvq_graph_end_capture(gpu, C.c_void_p(st.ptr), C.byref(exe)))
+_lib.check(_lib.lib().nvq_graph_launch(gpu, exe, C.c_void_p(st.ptr)))
+first = results()
+step()
+assert all(a.any() and np.array_equal(a, b) for a, b in zip(first, results()))
+print("same bits")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured(gpu):
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS.replace("{gpu}", str(gpu))], capture_output=True, text=True,
+                         timeout=300, cwd=Path(__file__).resolve().parents[1])
+    assert run.returncode == 0 and "same bits" in run.stdout, run.stderr
